@@ -302,6 +302,146 @@ int ligguf_cuda_matmul_reduce_async(const ligguf_qmat* w, ligguf_reduce* r, cons
 int ligguf_cuda_reduce_wait_async(ligguf_reduce* r, float* d_x_inout, float* d_out, void* stream);
 int ligguf_cuda_reduce_status(ligguf_reduce* r, void* stream);
 
+/* ---- long contexts: rotary positions ------------------------------------------------------ */
+/* No counterpart in the reference: additions for models with long contexts.  The reference rotates
+ * adjacent pairs of a head without scaling (fast/lil_math.cpp:901-920); these calls add the other
+ * pair layout, scaled frequencies, 16-bit rows and positions from device memory. */
+#define LIGGUF_ROPE_ADJACENT 0 /* pairs (2i, 2i+1), as the reference's rope() */
+#define LIGGUF_ROPE_HALVES 1   /* pairs (i, i + rope_dim/2) */
+#define LIGGUF_ROPE_SCALE_NONE 0   /* f_i = base^(-2i/rope_dim) */
+#define LIGGUF_ROPE_SCALE_LINEAR 1 /* f_i / factor */
+#define LIGGUF_ROPE_SCALE_BLEND 2  /* r = orig_context * f_i / (2 pi) turns within the trained context,
+                                      g = clamp((r - low) / (high - low), 0, 1):
+                                      f_i * (g + (1 - g) / factor) */
+typedef struct ligguf_rope_cfg {
+    int head_dim;      /* 64 or 128 */
+    int rope_dim;      /* leading elements of a head that are rotated: even, 0 (none) to head_dim */
+    int layout;        /* LIGGUF_ROPE_ADJACENT or _HALVES */
+    int scaling;       /* LIGGUF_ROPE_SCALE_* */
+    float base;        /* theta */
+    float factor;      /* scaled: >= 1 */
+    int orig_context;  /* BLEND: positions of the trained context */
+    float low, high;   /* BLEND: low < high */
+    float magnitude;   /* multiplies the rotated elements; 0 = 1 (0.1 ln(factor) + 1 for YaRN) */
+    const float* freq; /* optional host table of rope_dim/2 inverse frequencies, used as they are in
+                          place of base and scaling; NULL = computed */
+} ligguf_rope_cfg;
+
+/* RMS norm of every query and key head, then its rotation, in one pass over the rows:
+ *   y = x / sqrt(mean(x^2) + rms_epsilon) * gamma   (qk_norm), then each pair (a, b) of y at position p
+ *   becomes magnitude * (a cos(p f) - b sin(p f), a sin(p f) + b cos(p f)).
+ * The angle is formed in 64 bits, so a rotation keeps fp32 accuracy at any position; sums are fp32. */
+typedef struct ligguf_qk_rope_cfg {
+    ligguf_rope_cfg rope;
+    int n_heads;             /* query heads, at least 1 */
+    int n_kv_heads;          /* key heads; 0 = queries only */
+    int qk_norm;             /* 1 = norm before the rotation */
+    float rms_epsilon;
+    int in_type, out_type;   /* LIGGUF_KV_F32 / F16 / BF16 of the rows read and written */
+    long long q_stride, k_stride;         /* elements between tokens' rows (0 = heads * head_dim) */
+    long long q_out_stride, k_out_stride; /* same, of the rows written */
+    int device;
+} ligguf_qk_rope_cfg;
+typedef struct ligguf_qk_rope ligguf_qk_rope;
+int ligguf_cuda_qk_rope_init(const ligguf_qk_rope_cfg* cfg, ligguf_qk_rope** out);
+int ligguf_cuda_qk_rope_free(ligguf_qk_rope* h);
+/* n tokens (0 is a no-op) at positions pos0 + i, or d_pos[i] (device, not negative) when d_pos is not
+ * NULL.  Device pointers, rows 16-byte aligned (base and stride); d_q_gamma / d_k_gamma are head_dim
+ * floats each (qk_norm only).  In place (d_q_out == d_q, same type and stride) is allowed; other
+ * overlaps are not. */
+int ligguf_cuda_qk_rope_async(ligguf_qk_rope* h, int n, int pos0, const int* d_pos, const void* d_q,
+                              const void* d_k, const float* d_q_gamma, const float* d_k_gamma,
+                              void* d_q_out, void* d_k_out, void* stream);
+
+/* ---- long contexts: a cache of 4-bit keys and values -------------------------------------- */
+/* A handle holds, for n_layers layers and n_seqs sequences, n_context positions of keys (normed and
+ * rotated) and values in 4.5 bits: each 32 elements of a head are one block of GGUF's Q4_0 type:
+ * d = fp16(m / -8) with m the element of largest magnitude (the positive one of two), codes
+ * clamp(round(x / d) + 8, 0, 15), value (code - 8) * d.  |d| saturates at 65504; a block with an
+ * infinity or a NaN in it becomes NaN.  In HBM the codes lie in the order in which the attention
+ * kernel's matrix instructions take them; load / store convert from and to blocks.
+ * One call at a time: the calls of one handle must not overlap on the GPU. */
+typedef struct ligguf_kv4_cfg {
+    ligguf_rope_cfg rope;
+    int n_layers, n_seqs, n_context;
+    int n_heads, n_kv_heads; /* n_heads / n_kv_heads: 1, 2, 4 or 8 */
+    int qk_norm;             /* 1 = per-head RMS norm of q and k before the rotation */
+    float rms_epsilon;
+    int window;              /* a query at p sees keys in (p - window, p] ... (0 = all of [0, p]) */
+    int sinks;               /* ... and the first `sinks` keys whatever the window */
+    float scale;             /* of the scores; 0 = 1 / sqrt(head_dim) */
+    int in_type;             /* LIGGUF_KV_* of q, k, v and of decode's out */
+    int rows_type;           /* LIGGUF_KV_* of append's q_out and of all k_rows / v_rows */
+    long long q_stride, k_stride, v_stride; /* elements between tokens' rows of q, k, v (0 = packed) */
+    int device;
+} ligguf_kv4_cfg;
+typedef struct ligguf_kv4 ligguf_kv4;
+int ligguf_cuda_kv4_init(const ligguf_kv4_cfg* cfg, ligguf_kv4** out);
+int ligguf_cuda_kv4_free(ligguf_kv4* h);
+/* One layer's norm weights, head_dim floats each (host), before its first append or decode with qk_norm. */
+int ligguf_cuda_kv4_set_qk_norm(ligguf_kv4* h, int layer, const float* q_gamma, const float* k_gamma);
+/* A prompt's n tokens (0 is a no-op) at positions [pos0, pos0 + n) of sequence seq: norms and rotates q
+ * and k, quantizes k and v into the cache, and writes, where the pointer is not NULL, the queries
+ * (q_out [n][n_heads*head_dim]) and the rows as the cache now holds them (k_rows, v_rows
+ * [n][n_kv_heads*head_dim]) in rows_type, packed.  d_q may be NULL when q_out is.  Device pointers, rows 16-byte
+ * aligned (base and stride), enqueued on `stream`. */
+int ligguf_cuda_kv4_append_async(ligguf_kv4* h, int layer, int seq, int pos0, int n, const void* d_q,
+                                 const void* d_k, const void* d_v, void* d_q_out, void* d_k_rows,
+                                 void* d_v_rows, void* stream);
+/* One token of each of the first n_rows sequences, at position `pos`, or d_pos[r] (device) when d_pos is
+ * not NULL: norms and rotates q and k, appends k and v, and attends over the sequence's visible cached
+ * positions below its own and its own unquantized k, v (as the engine's decode takes the current token,
+ * fast/ligguf_fast_qk.cpp:77-78,98-99).  d_pos[r] < 0: an idle row, zeros in out (and k_rows, v_rows),
+ * nothing appended.  d_pos[r] >= n_context: the same, and reported by ligguf_cuda_kv4_status.
+ *   q [n_rows][n_heads*head_dim], k, v [n_rows][n_kv_heads*head_dim] in in_type (rows by the strides);
+ *   out [n_rows][n_heads*head_dim] in in_type, packed; k_rows, v_rows: NULL, or the appended rows as the
+ *   cache holds them, for a mirror of the cache. */
+int ligguf_cuda_kv4_decode_async(ligguf_kv4* h, int layer, int n_rows, int pos, const int* d_pos,
+                                 const void* d_q, const void* d_k, const void* d_v, void* d_out,
+                                 void* d_k_rows, void* d_v_rows, void* stream);
+/* Positions [pos0, pos0 + n) of sequence seq as rows of rows_type (either pointer may be NULL). */
+int ligguf_cuda_kv4_read_async(ligguf_kv4* h, int layer, int seq, int pos0, int n, void* d_k_rows,
+                               void* d_v_rows, void* stream);
+/* The same positions of sequences [seq0, seq0 + n_seqs) as Q4_0 blocks, [n_seqs][n][n_kv_heads*head_dim/32]
+ * of 18 bytes {fp16 d; 16 bytes, byte i = code i | code (i+16) << 4} for keys and values (device memory,
+ * 2-byte aligned): into the cache, or out of it, bit for bit. */
+int ligguf_cuda_kv4_load_async(ligguf_kv4* h, int layer, int seq0, int n_seqs, int pos0, int n,
+                               const void* d_k_blocks, const void* d_v_blocks, void* stream);
+int ligguf_cuda_kv4_store_async(ligguf_kv4* h, int layer, int seq0, int n_seqs, int pos0, int n,
+                                void* d_k_blocks, void* d_v_blocks, void* stream);
+/* Waits for `stream`, then: LIGGUF_ATTN_EINVAL if a decode since the last status call met a position
+ * beyond n_context, LIGGUF_ATTN_ETIMEDOUT if a bounded in-kernel wait gave up, else 0. */
+int ligguf_cuda_kv4_status(ligguf_kv4* h, void* stream);
+
+/* ---- long contexts: windowed attention over 16-bit rows ------------------------------------ */
+/* Causal attention of n queries a sequence over m rows of keys and values, with a sliding window and
+ * first tokens ("sinks") that stay visible.  Query i of batch entry b is at position p = pos0[b] + i; key
+ * j (row j, position j) is seen iff j <= p, j < lens[b], and window == 0 or j > p - window or j < sinks.
+ * A query that sees no key gets zeros.  Rows of k and v at or beyond lens[b] may hold anything. */
+typedef struct ligguf_window_cfg {
+    int n_heads, n_kv_heads, head_dim; /* any whole n_heads / n_kv_heads; head_dim 64 or 128 */
+    int window, sinks;                 /* window 0 = plain causal */
+    float scale;                       /* of the scores; 0 = 1 / sqrt(head_dim) */
+    int in_type;                       /* LIGGUF_KV_F16 or _BF16 */
+    int out_type;                      /* in_type or LIGGUF_KV_F32 */
+    long long q_stride, k_stride, v_stride; /* elements between rows (0 = packed) */
+    long long q_batch_stride, k_batch_stride, v_batch_stride; /* between entries (0 = n or m rows) */
+    int device;
+} ligguf_window_cfg;
+typedef struct ligguf_window ligguf_window;
+int ligguf_cuda_window_init(const ligguf_window_cfg* cfg, ligguf_window** out);
+int ligguf_cuda_window_free(ligguf_window* h);
+/* Device pointers, rows 16-byte aligned (base and strides); out [batch][n][n_heads*head_dim], packed.
+ * d_lens NULL: m keys each; d_pos0 NULL: the queries are each sequence's last (lens[b] - n + i).  batch
+ * or n of 0 is a no-op.  The products' operands are in_type (so are the weights of the sum over v,
+ * rounded once), accumulated in fp32.  The calls of one handle must not overlap on the GPU. */
+int ligguf_cuda_window_attn_async(ligguf_window* h, int batch, int n, int m, const void* d_q,
+                                  const void* d_k, const void* d_v, const int* d_pos0,
+                                  const int* d_lens, void* d_out, void* stream);
+/* Waits for `stream`, then LIGGUF_ATTN_ETIMEDOUT if a bounded in-kernel wait gave up since the last
+ * status call, else 0. */
+int ligguf_cuda_window_status(ligguf_window* h, void* stream);
+
 /* ---- seeded synthetic inputs ------------------------------------------------------------- */
 /* Tensor ids of the synthetic generator's streams. */
 #define LIGGUF_SYNTH_K 1

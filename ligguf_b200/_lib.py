@@ -16,8 +16,11 @@ KV_F32, KV_F16, KV_BF16 = 0, 1, 2
 SCALE_MUL, SCALE_DIV = 0, 1
 MODE_SIMT, MODE_TC = 0, 1
 SYNTH_K, SYNTH_V, SYNTH_Q, SYNTH_KNEW, SYNTH_VNEW, SYNTH_QGAMMA, SYNTH_KGAMMA = 1, 2, 3, 4, 5, 6, 7
+ROPE_ADJACENT, ROPE_HALVES = 0, 1
+ROPE_SCALE_NONE, ROPE_SCALE_LINEAR, ROPE_SCALE_BLEND = 0, 1, 2
 NOALLOC_MAX_ELEMS = 1 << 22  # LIGGUF_NOALLOC_MAX_ELEMS
 
+_ll = ctypes.c_longlong
 _i, _f, _u64, _sz, _vp, _cp = ctypes.c_int, ctypes.c_float, ctypes.c_uint64, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_char_p
 
 
@@ -41,6 +44,38 @@ class AttnCfg(ctypes.Structure):
         ("kv_head0", _i),
         ("kv_headn", _i),
     ]
+
+
+class RopeCfg(ctypes.Structure):
+    """Mirror of ``ligguf_rope_cfg``."""
+
+    _fields_ = [("head_dim", _i), ("rope_dim", _i), ("layout", _i), ("scaling", _i), ("base", _f), ("factor", _f),
+                ("orig_context", _i), ("low", _f), ("high", _f), ("magnitude", _f), ("freq", ctypes.POINTER(_f))]
+
+
+class QkRopeCfg(ctypes.Structure):
+    """Mirror of ``ligguf_qk_rope_cfg``."""
+
+    _fields_ = [("rope", RopeCfg), ("n_heads", _i), ("n_kv_heads", _i), ("qk_norm", _i), ("rms_epsilon", _f),
+                ("in_type", _i), ("out_type", _i), ("q_stride", _ll), ("k_stride", _ll), ("q_out_stride", _ll),
+                ("k_out_stride", _ll), ("device", _i)]
+
+
+class Kv4Cfg(ctypes.Structure):
+    """Mirror of ``ligguf_kv4_cfg``."""
+
+    _fields_ = [("rope", RopeCfg), ("n_layers", _i), ("n_seqs", _i), ("n_context", _i), ("n_heads", _i),
+                ("n_kv_heads", _i), ("qk_norm", _i), ("rms_epsilon", _f), ("window", _i), ("sinks", _i), ("scale", _f),
+                ("in_type", _i), ("rows_type", _i), ("q_stride", _ll), ("k_stride", _ll), ("v_stride", _ll),
+                ("device", _i)]
+
+
+class WindowCfg(ctypes.Structure):
+    """Mirror of ``ligguf_window_cfg``."""
+
+    _fields_ = [("n_heads", _i), ("n_kv_heads", _i), ("head_dim", _i), ("window", _i), ("sinks", _i), ("scale", _f),
+                ("in_type", _i), ("out_type", _i), ("q_stride", _ll), ("k_stride", _ll), ("v_stride", _ll),
+                ("q_batch_stride", _ll), ("k_batch_stride", _ll), ("v_batch_stride", _ll), ("device", _i)]
 
 
 class LigGufAttnError(RuntimeError):
@@ -92,6 +127,22 @@ _PROTOS = {
     "ligguf_cuda_matmul3_batch": [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp],
     "ligguf_cuda_quantize_q8_K_async": [_vp, _i, _vp, _vp],
     "ligguf_cuda_quantize_q8_0_async": [_vp, _i, _vp, _vp],
+    "ligguf_cuda_qk_rope_init": [ctypes.POINTER(QkRopeCfg), ctypes.POINTER(_vp)],
+    "ligguf_cuda_qk_rope_free": [_vp],
+    "ligguf_cuda_qk_rope_async": [_vp, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "ligguf_cuda_kv4_init": [ctypes.POINTER(Kv4Cfg), ctypes.POINTER(_vp)],
+    "ligguf_cuda_kv4_free": [_vp],
+    "ligguf_cuda_kv4_set_qk_norm": [_vp, _i, _vp, _vp],
+    "ligguf_cuda_kv4_append_async": [_vp, _i, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "ligguf_cuda_kv4_decode_async": [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "ligguf_cuda_kv4_read_async": [_vp, _i, _i, _i, _i, _vp, _vp, _vp],
+    "ligguf_cuda_kv4_load_async": [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp],
+    "ligguf_cuda_kv4_store_async": [_vp, _i, _i, _i, _i, _i, _vp, _vp, _vp],
+    "ligguf_cuda_kv4_status": [_vp, _vp],
+    "ligguf_cuda_window_init": [ctypes.POINTER(WindowCfg), ctypes.POINTER(_vp)],
+    "ligguf_cuda_window_free": [_vp],
+    "ligguf_cuda_window_attn_async": [_vp, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp, _vp],
+    "ligguf_cuda_window_status": [_vp, _vp],
     "ligguf_cuda_synth_fill": [_vp, _i, _sz, _u64, _u64, _u64, _f, _f, _vp],
 }
 
