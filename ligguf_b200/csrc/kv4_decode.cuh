@@ -1,4 +1,33 @@
-// kv4_decode.cuh - one token of each sequence over the 4-bit cache.
+// kv4_decode.cuh - one token of each sequence: norm, rotation, append, attention over the 4-bit cache.
+//
+//   out_h = sum_j w_j v_j / sum_j w_j,  w_j = 2^(x_j),  x_j = log2(e) * scale * (q_h . k_j)
+//
+// over the visible cached positions j and the token's own unquantized k, v.
+//
+// Bound by the cache's bytes (18 D a tile of 16 positions and KV head) as long as the arithmetic on them
+// stays short, so both products run on the tensor cores (mma.m16n8k16, fp16 operands, fp32 sums) straight
+// from the packed codes:
+//   - A code n (0..15) masked into the low mantissa bits of a half is the subnormal n * 2^-24, and shifted
+//     by a nibble n * 2^-20: exact operands that cost one AND for two codes.  The powers of two are taken
+//     out of the fp32 results; the -8 of (n - 8) d enters as the products' initial value (keys) or is
+//     subtracted once at the end (values).
+//   - S^T = K Q^T: 16 positions x 8 columns.  The key scales multiply the fp32 sums of their 32 elements.
+//   - Queries and weights are split into two halves each, hi + lo, which together hold 22 bits, so the
+//     results are those of fp32 arithmetic.  Up to four query heads a KV head share one product: columns
+//     0-3 are the hi parts of the heads, 4-7 the lo parts, which cost nothing then.  With eight heads the
+//     lo parts are a second product into the same sums.
+//   - O^T += V^T W: the value scales are multiplied into the weights, one B operand for each 32 elements.
+//     The weights go from the sums' layout to the operand's by transposing 8x8 fragments (movmatrix).
+//   - Weights carry value scales of any size, so the running maximum is that of x_j + (exponent of the
+//     largest scale of row j): |weight * scale| stays in [0, 2^15] of fp16's range whatever the scales.
+//     It is only moved when a row exceeds it by 2^8, a vote of the warp per tile.
+//
+// The work is one list: (row, KV head) items, each its visible tiles and one unit more for the token
+// itself, cut into equal contiguous shares of as many blocks as fit at once, whatever the lengths of the
+// sequences; the cut is computed by every block from the positions, which may be in device memory.  In a
+// share, the 8 warps take tiles in turn, each with its own ring of bulk copies and its own running sums,
+// which the block joins per item.  Items that several blocks share are joined by the last of them to
+// finish, in the order of the blocks, so results repeat bit for bit.
 #pragma once
 
 #include "kv4.cuh"
@@ -15,177 +44,700 @@ struct Kv4DecodeArgs {
     const double* turns;
     const int* pos_rows;
     int pos, n_rows, q_heads, kv_heads, pairs, norm, n_context, layout, rows_type;
-    float eps, magnitude, scale;
+    float eps, magnitude, scale_log2;
     int window, sinks;
     uint8_t* tiles;  // first tile of (layer, sequence 0, head 0)
     long long tiles_per_head;
+    float* parts;    // [blocks][2] partial results
+    int* tickets;    // [n_rows * kv_heads], zero between calls
     int* err;
 };
 
 // Error word of the status call, beside the waits' codes: a decode position beyond the context.
 enum : int { KERR_POSITION = 16 };
 
-// One head's 8 elements a lane (D/8 lanes, the same in every group of lanes): norm and rotation.
-template <int D>
-__device__ __forceinline__ void rope_head8(float (&x)[8], int l, const float* gamma, int norm, float eps,
-                                           const float2* cs, int pairs, int layout, float* xs) {
+constexpr int kKv4Warps = 8;
+constexpr int kKv4Threads = 32 * kKv4Warps;
+constexpr int kKv4MinUnits = kKv4Warps;  // tiles a block has at least: fewer blocks share a short context
+
+// Floats of one partial result: o [NREP][D], m [NREP], l [NREP].
+__host__ __device__ constexpr int kv4_part_floats(int nrep, int dim) { return nrep * (dim + 2); }
+
+template <int D, int NREP>
+struct Kv4DecodeSmem {
+    static constexpr int kStages = D == 128 ? 4 : 8;
+    static constexpr size_t kRing = 0;
+    static constexpr size_t kQ = kRing + size_t(kKv4Warps) * kStages * Kv4<D>::kTileBytes;
+    static constexpr size_t kKn = kQ + NREP * D * 4;
+    static constexpr size_t kVn = kKn + D * 4;
+    static constexpr size_t kCs = kVn + D * 4;
+    static constexpr size_t kO = kCs + D / 2 * 8;                           // [warps][NREP][D]
+    static constexpr size_t kM = kO + size_t(kKv4Warps) * NREP * D * 4;     // [warps + 1][NREP]
+    static constexpr size_t kL = kM + (kKv4Warps + 1) * NREP * 4;
+    static constexpr size_t kBar = (kL + (kKv4Warps + 1) * NREP * 4 + 7) / 8 * 8;
+    static constexpr size_t kMisc = kBar + kKv4Warps * kStages * 8;
+    static constexpr size_t kTotal = kMisc + 16;
+};
+
+// Visible cached tiles of a row at position p: tiles [0, ns) hold the sinks, [tw, tw + nt - ns) the window.
+struct Kv4Row {
+    int pos, first, sinks;  // keys j < pos with j >= first or j < sinks
+    int ns, tw, nt;
+};
+__device__ __forceinline__ Kv4Row kv4_row(const Kv4DecodeArgs& a, int pos) {
+    Kv4Row r;
+    r.pos = pos;
+    r.first = a.window && pos >= a.window ? pos - a.window + 1 : 0;
+    r.sinks = min(a.sinks, r.first);
+    r.tw = r.first / kKv4Tile;
+    r.ns = min((r.sinks + kKv4Tile - 1) / kKv4Tile, r.tw);
+    r.nt = r.ns + (pos + kKv4Tile - 1) / kKv4Tile - min(r.tw, (pos + kKv4Tile - 1) / kKv4Tile);
+    return r;
+}
+__device__ __forceinline__ int kv4_tile_of(const Kv4Row& r, int i) { return i < r.ns ? i : r.tw + (i - r.ns); }
+// Units of one head of a row: its tiles and the token itself; none for an idle row.
+__device__ __forceinline__ long long kv4_units(const Kv4DecodeArgs& a, int pos) {
+    return pos < 0 || pos >= a.n_context ? 0 : kv4_row(a, pos).nt + 1;
+}
+__device__ __forceinline__ int kv4_pos(const Kv4DecodeArgs& a, int r) { return a.pos_rows ? __ldg(a.pos_rows + r) : a.pos; }
+
+// The row (returned) whose units hold unit u of the whole list, and the first of its units; n_rows if none.
+// Warp-collective.
+__device__ __forceinline__ int kv4_find_row(const Kv4DecodeArgs& a, long long u, long long& start, int lane) {
+    if (!a.pos_rows) {
+        const long long per = kv4_units(a, a.pos) * a.kv_heads;
+        const int r = per ? static_cast<int>(u / per) : a.n_rows;
+        start = r * per;
+        return r;
+    }
+    long long before = 0;
+    for (int r0 = 0; r0 < a.n_rows; r0 += 32) {
+        const long long mine = r0 + lane < a.n_rows ? kv4_units(a, a.pos_rows[r0 + lane]) * a.kv_heads : 0;
+        long long upto = mine;  // inclusive scan
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        const unsigned past = __ballot_sync(0xffffffffu, before + upto > u);
+        if (past) {
+            const int w = __ffs(past) - 1;
+            start = before + __shfl_sync(0xffffffffu, upto - mine, w);
+            return r0 + w;
+        }
+        before += __shfl_sync(0xffffffffu, upto, 31);
+    }
+    start = before;
+    return a.n_rows;
+}
+__device__ __forceinline__ long long kv4_total(const Kv4DecodeArgs& a, int lane) {
+    if (!a.pos_rows) return kv4_units(a, a.pos) * a.kv_heads * a.n_rows;
+    long long n = 0;
+    for (int r = lane; r < a.n_rows; r += 32) n += kv4_units(a, a.pos_rows[r]);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+    return n * a.kv_heads;
+}
+
+// One head (8 elements a lane, D/8 lanes, the other lanes the same again): norm and rotation; `dst`
+// (shared, D floats) carries the exchange and gets the result.
+template <typename In, int D>
+__device__ __forceinline__ void kv4_head(const In* src, const float* gamma, bool norm, float eps, const float2* cs,
+                                         int pairs, int layout, float* dst, float (&x)[8], int lane) {
+    constexpr int L = D / 8;
+    const int l = lane % L;
+    load8(src + l * 8, x);
     if (norm) {
+        float g[8];
+        load8(gamma + l * 8, g);
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-        ss = head_sum<D / 8>(ss);
+        ss = head_sum<L>(ss);
         const float rs = 1.0f / sqrtf(ss / static_cast<float>(D) + eps);
-        float g[8];
-        load8(gamma + l * 8, g);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = (x[i] * rs) * g[i];
     }
-    const int group = (threadIdx.x & 31) / (D / 8);
-    __syncwarp();
+    if (layout == LIGGUF_ROPE_ADJACENT) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) xs[group * D + l * 8 + i] = x[i];
-    __syncwarp();
+        for (int i = 0; i < 4; ++i)
+            if (4 * l + i < pairs) {
+                const float2 w = cs[4 * l + i];
+                const float x0 = x[2 * i], x1 = x[2 * i + 1];
+                x[2 * i] = x0 * w.x - x1 * w.y;
+                x[2 * i + 1] = x0 * w.y + x1 * w.x;
+            }
+    } else {
+        if (lane < L) store8(dst + l * 8, x);
+        __syncwarp();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int e = 8 * l + i;
-        if (e < 2 * pairs) {
-            const bool low = layout == 0 ? !(e & 1) : e < pairs;
-            const int other = layout == 0 ? e ^ 1 : low ? e + pairs : e - pairs;
-            const float2 w = cs[layout == 0 ? e >> 1 : low ? e : e - pairs];
-            x[i] = x[i] * w.x + (low ? -xs[group * D + other] : xs[group * D + other]) * w.y;
+        for (int i = 0; i < 8; ++i) {
+            const int e = 8 * l + i;
+            if (e < 2 * pairs) {
+                const bool low = e < pairs;
+                const float2 w = cs[low ? e : e - pairs];
+                const float other = dst[low ? e + pairs : e - pairs];
+                x[i] = x[i] * w.x + (low ? -other : other) * w.y;
+            }
         }
+        __syncwarp();
     }
-    __syncwarp();
 }
 
-template <typename T>
 __device__ __forceinline__ void store_rows8(void* rows, int type, long long at, const float (&y)[8]) {
-    if (type == 0)
+    if (type == LIGGUF_KV_F32)
         store8(static_cast<float*>(rows) + at, y);
-    else if (type == 1)
+    else if (type == LIGGUF_KV_F16)
         store8(static_cast<__half*>(rows) + at, y);
     else
         store8(static_cast<__nv_bfloat16*>(rows) + at, y);
 }
 
-// Block (KV head, row): 8 warps walk the visible positions in turn, one position at a time, each with its
-// own running maximum and sums; then they are joined.
-template <typename In, int D, int NREP>
-__global__ void __launch_bounds__(256) kv4_decode_kernel(const Kv4DecodeArgs a) {
-    constexpr int L = D / 8;
-    __shared__ float2 cs[D / 2];
-    __shared__ float qs[NREP][D], kn[D], vn[D], xs[8][256];
-    __shared__ float wm[8][NREP], wl[8][NREP], wo[8][NREP][D];
-    const int g = blockIdx.x, r = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int pos = a.pos_rows ? a.pos_rows[r] : a.pos;
-    const bool over = pos >= a.n_context;
-    const int l = lane % L;
-    uint8_t* head_tiles = a.tiles + (static_cast<long long>(r) * a.kv_heads + g) * a.tiles_per_head * Kv4<D>::kTileBytes;
-    In* out = static_cast<In*>(a.out) + (static_cast<long long>(r) * a.q_heads + g * NREP) * D;
-    if (pos < 0 || over) {
-        if (over && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = KERR_POSITION;
-        const float z[8] = {};
-        for (int u = threadIdx.x; u < NREP * L; u += 256) store8(out + u * 8, z);
-        if (threadIdx.x < L) {
-            const long long at = (static_cast<long long>(r) * a.kv_heads + g) * D + threadIdx.x * 8;
-            if (a.k_rows) store_rows8<In>(a.k_rows, a.rows_type, at, z);
-            if (a.v_rows) store_rows8<In>(a.v_rows, a.rows_type, at, z);
-        }
-        return;
-    }
-    for (int i = threadIdx.x; i < a.pairs; i += 256) cs[i] = rope_turn(a.turns, i, pos, a.magnitude);
-    __syncthreads();
-    for (int job = warp; job < NREP + 2; job += 8) {
-        const bool isq = job < NREP;
-        const In* src = isq         ? static_cast<const In*>(a.q) + r * a.q_stride + (g * NREP + job) * D
-                        : job == NREP ? static_cast<const In*>(a.k) + r * a.k_stride + g * D
-                                      : static_cast<const In*>(a.v) + r * a.v_stride + g * D;
-        float x[8];
-        load8(src + l * 8, x);
-        if (job <= NREP) rope_head8<D>(x, l, isq ? a.q_gamma : a.k_gamma, a.norm, a.eps, cs, a.pairs, a.layout, xs[warp]);
-        float* dst = isq ? qs[job] : job == NREP ? kn : vn;
-        if (lane < L)
+// D = A B + C: m16n8k16, fp16 operands, fp32 sums.
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1, float c0, float c1, float c2, float c3) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint2 lds64(const void* p) {
+    uint2 r;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.x), "=r"(r.y) : "r"(smem_u32(p)));
+    return r;
+}
+
+// Sum over the 8 lanes (row groups) that share a fragment's column pair.
+__device__ __forceinline__ float rows_sum(float v) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dst[l * 8 + i] = x[i] * (isq ? a.scale : 1.f);
-        if (!isq) {
-            uint32_t codes;
-            const __half d = kv4_quantize8(x, codes);
-            if (lane < L) {
-                uint8_t* tile = head_tiles + static_cast<long long>(pos / kKv4Tile) * Kv4<D>::kTileBytes;
-                if (job == NREP)
-                    kv4_store8<D, false>(tile, pos % kKv4Tile, l, codes, d);
-                else
-                    kv4_store8<D, true>(tile, pos % kKv4Tile, l, codes, d);
-                void* rows = job == NREP ? a.k_rows : a.v_rows;
-                if (rows) {
-                    float y[8];
-                    kv4_values8(codes, d, y);
-                    store_rows8<In>(rows, a.rows_type, (static_cast<long long>(r) * a.kv_heads + g) * D + l * 8, y);
+    for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// One warp's running sums over the tiles it takes of an item.
+template <int D, int NREP>
+struct Kv4Warp {
+    static constexpr bool kWide = NREP > 4;  // hi and lo parts as two products
+    static constexpr int KS = D / 16, G = D / 32;
+    uint32_t b[kWide ? 2 : 1][KS][2];  // queries, as B operands
+    float c[kWide ? 2 : 1][G][2];      // -8 * sum of a group's queries, of this lane's columns
+    float sx[2];                       // scales of the scores of this lane's two heads
+    float m[2], l[2], ws[G][2];        // running maxima, sums of weights and of weights * value scales
+    float o[KS][4];
+
+    // q: [NREP][D] in shared memory, times scale * log2(e).
+    __device__ __forceinline__ void start(const float* q, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        const int head = kWide ? g : g & 3;
+        const bool is_lo = !kWide && g >= 4;
+        float top = 0.f;
+        float4 x[KS];
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+            x[j] = head < NREP ? *reinterpret_cast<const float4*>(q + head * D + 16 * j + 4 * t) : make_float4(0.f, 0.f, 0.f, 0.f);
+            top = fmaxf(top, fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w))));
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // A power of two that brings the head's largest element to [2^10, 2^11): hi is then a normal half
+        // and lo loses nothing either.
+        const int e = min(100, max(-100, ((__float_as_int(top) >> 23) & 255) - 127));
+        const float up = __int_as_float((127 + 10 - e) << 23);
+        float sum[2][G] = {};
+#pragma unroll
+        for (int j = 0; j < KS; ++j) {
+            const float v[4] = {x[j].x * up, x[j].y * up, x[j].z * up, x[j].w * up};
+            uint32_t part[2][2];
+#pragma unroll
+            for (int p = 0; p < 2; ++p) {  // columns 2t + b: elements 4t + 2b (codes * 2^-24), 4t + 2b + 1 (* 2^-20)
+                const float f = p ? 0.0625f : 1.f;
+                const uint32_t hi = pack_f16(v[p] * f, v[2 + p] * f);
+                const float2 h = unpack_f16(hi);
+                const uint32_t lo = pack_f16(v[p] * f - h.x, v[2 + p] * f - h.y);
+                const float2 r = unpack_f16(lo);
+                part[0][p] = hi;
+                part[1][p] = lo;
+                sum[0][j / 2] += (h.x + h.y) * (p ? 16.f : 1.f);
+                sum[1][j / 2] += (r.x + r.y) * (p ? 16.f : 1.f);
+            }
+            if constexpr (kWide) {
+                b[0][j][0] = part[0][0], b[0][j][1] = part[0][1];
+                b[1][j][0] = part[1][0], b[1][j][1] = part[1][1];
+            } else {
+                b[0][j][0] = is_lo ? part[1][0] : part[0][0];
+                b[0][j][1] = is_lo ? part[1][1] : part[0][1];
+            }
+        }
+        // The sums of a column lie in the four lanes of its row group; this lane's columns are 2t, 2t+1.
+#pragma unroll
+        for (int p = 0; p < (kWide ? 2 : 1); ++p)
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                float s = kWide ? sum[p][i] : (is_lo ? sum[1][i] : sum[0][i]);
+                s += __shfl_xor_sync(0xffffffffu, s, 1);
+                s += __shfl_xor_sync(0xffffffffu, s, 2);
+                s *= -8.f / 16777216.f;
+                c[p][i][0] = __shfl_sync(0xffffffffu, s, 8 * t);
+                c[p][i][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+            }
+        const float down = __int_as_float((127 + e + 14) << 23);  // 2^(e - 10) * 2^24
+        sx[0] = __shfl_sync(0xffffffffu, down, 8 * t);
+        sx[1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) m[i] = -1e30f, l[i] = 0.f;
+#pragma unroll
+        for (int i = 0; i < G; ++i) ws[i][0] = ws[i][1] = 0.f;
+#pragma unroll
+        for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    }
+
+    // One tile in shared memory; positions k0 + row.
+    __device__ __forceinline__ void tile(const uint8_t* tp, const Kv4Row& r, int k0, int lane) {
+        const int g = lane >> 2;
+        // Scores of positions g (x[0], x[1]) and g + 8 (x[2], x[3]) with this lane's columns.
+        float x[4] = {0.f, 0.f, 0.f, 0.f};
+        {
+            float ks[2][G];
+            load_scales(tp + Kv4<D>::kKeyScales, g, ks);
+#pragma unroll
+            for (int ch = 0; ch < D / 64; ++ch) {
+                const uint4 w4 = lds128(tp + ch * 512 + lane * 16);
+                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+                for (int gr = 0; gr < 2; ++gr) {
+                    const int i = ch * 2 + gr;
+                    float s[4] = {c[0][i][0], c[0][i][1], c[0][i][0], c[0][i][1]};
+                    if constexpr (kWide) s[0] += c[1][i][0], s[1] += c[1][i][1], s[2] += c[1][i][0], s[3] += c[1][i][1];
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const int j = 2 * i + u;
+                        const uint32_t lo = w[2 * gr + u], hi = lo >> 8;
+                        const uint32_t a0 = lo & 0x000F000Fu, a2 = lo & 0x00F000F0u, a1 = hi & 0x000F000Fu, a3 = hi & 0x00F000F0u;
+                        mma_f16(s, a0, a1, a2, a3, b[0][j][0], b[0][j][1], s[0], s[1], s[2], s[3]);
+                        if constexpr (kWide) mma_f16(s, a0, a1, a2, a3, b[1][j][0], b[1][j][1], s[0], s[1], s[2], s[3]);
+                    }
+                    x[0] = fmaf(s[0], ks[0][i], x[0]);
+                    x[1] = fmaf(s[1], ks[0][i], x[1]);
+                    x[2] = fmaf(s[2], ks[1][i], x[2]);
+                    x[3] = fmaf(s[3], ks[1][i], x[3]);
+                }
+            }
+        }
+        if constexpr (!kWide) {  // hi and lo columns of a head lie two lanes apart; both get the sum
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], 2);
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] *= sx[i & 1];
+        float vs[2][G];
+        const float2 ex = load_value_scales(tp + Kv4<D>::kValueScales, g, vs);
+        if (k0 + kKv4Tile > r.pos || k0 < r.first) {
+            const int j0 = k0 + g, j1 = j0 + 8;
+            const bool s0 = j0 < r.pos && (j0 >= r.first || j0 < r.sinks);
+            const bool s1 = j1 < r.pos && (j1 >= r.first || j1 < r.sinks);
+            if (!s0) x[0] = x[1] = -INFINITY;
+            if (!s1) x[2] = x[3] = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < G; ++i) {  // an unseen row's scales may be anything: 0 * NaN is NaN
+                if (!s0) vs[0][i] = 0.f;
+                if (!s1) vs[1][i] = 0.f;
+            }
+        }
+        const float y[4] = {x[0] + ex.x, x[1] + ex.x, x[2] + ex.y, x[3] + ex.y};
+        const float t0 = fmaxf(y[0], y[2]), t1 = fmaxf(y[1], y[3]);
+        if (__any_sync(0xffffffffu, t0 > m[0] + 8.f || t1 > m[1] + 8.f)) move_max(t0, t1);
+        float p[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = ex2(x[i] - m[i & 1] + 7.f);
+        l[0] += p[0] + p[2];
+        l[1] += p[1] + p[3];
+        const float lo_lane = (lane & 2) ? -1.f : 0.f;
+#pragma unroll
+        for (int ch = 0; ch < D / 64; ++ch) {
+            const uint4 w4 = lds128(tp + Kv4<D>::kCodes + ch * 512 + lane * 16);
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+            for (int gr = 0; gr < 2; ++gr) {
+                const int i = ch * 2 + gr;
+                const float v0 = p[0] * vs[0][i], v1 = p[1] * vs[0][i], v2 = p[2] * vs[1][i], v3 = p[3] * vs[1][i];
+                ws[i][0] += v0 + v2;
+                ws[i][1] += v1 + v3;
+                uint32_t b0 = pack_f16(v0, v1), b1 = pack_f16(v2, v3);  // rows g, g + 8; this lane's columns
+                const float2 h0 = unpack_f16(b0), h1 = unpack_f16(b1);
+                uint32_t c0 = 0, c1 = 0;
+                if constexpr (kWide) {
+                    c0 = movmatrix(pack_f16(v0 - h0.x, v1 - h0.y));
+                    c1 = movmatrix(pack_f16(v2 - h1.x, v3 - h1.y));
+                } else {  // lanes of the lo columns hand over what the hi columns' rounding left
+                    b0 = pack_f16(fmaf(h0.x, lo_lane, v0), fmaf(h0.y, lo_lane, v1));
+                    b1 = pack_f16(fmaf(h1.x, lo_lane, v2), fmaf(h1.y, lo_lane, v3));
+                }
+                b0 = movmatrix(b0);
+                b1 = movmatrix(b1);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const int j = 2 * i + u;
+                    const uint32_t lo = w[2 * gr + u], hi = lo >> 8;
+                    const uint32_t a0 = lo & 0x000F000Fu, a1 = lo & 0x00F000F0u, a2 = hi & 0x000F000Fu, a3 = hi & 0x00F000F0u;
+                    mma_f16(o[j], a0, a1, a2, a3, b0, b1, o[j][0], o[j][1], o[j][2], o[j][3]);
+                    if constexpr (kWide) mma_f16(o[j], a0, a1, a2, a3, c0, c1, o[j][0], o[j][1], o[j][2], o[j][3]);
                 }
             }
         }
     }
-    __syncthreads();
-    constexpr int E = D / 32;
-    float m[NREP], ls[NREP], o[NREP][E];
+
+    // Moves the running maxima to those of all rows and rescales the sums.
+    __device__ __forceinline__ void move_max(float t0, float t1) {
 #pragma unroll
-    for (int h = 0; h < NREP; ++h) {
-        m[h] = -INFINITY, ls[h] = 0.f;
+        for (int s = 4; s < 32; s <<= 1) {
+            t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, s));
+            t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, s));
+        }
+        const float n0 = fmaxf(m[0], t0), n1 = fmaxf(m[1], t1);
+        const float f0 = ex2(m[0] - n0), f1 = ex2(m[1] - n1);
+        m[0] = n0, m[1] = n1;
+        l[0] *= f0, l[1] *= f1;
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[h][e] = 0.f;
+        for (int i = 0; i < G; ++i) ws[i][0] *= f0, ws[i][1] *= f1;
+#pragma unroll
+        for (int j = 0; j < KS; ++j) o[j][0] *= f0, o[j][1] *= f1, o[j][2] *= f0, o[j][3] *= f1;
     }
-    const int first = a.window && pos - a.window + 1 > 0 ? pos - a.window + 1 : 0;
-    const int sinks = a.window ? min(a.sinks, first) : 0;
-    const int count = sinks + (pos - first) + 1;  // the last is the token itself
-    for (int i = warp; i < count; i += 8) {
-        const int j = i < sinks ? i : first + (i - sinks);
-        float kx[E], vx[E];
-        if (i == count - 1) {
+
+    __device__ __forceinline__ static void load_scales(const uint8_t* s, int g, float (&out)[2][G]) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) kx[e] = kn[lane * E + e], vx[e] = vn[lane * E + e];
-        } else {
-            const uint8_t* tile = head_tiles + static_cast<long long>(j / kKv4Tile) * Kv4<D>::kTileBytes;
-            const int p = j % kKv4Tile;
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int el = lane * E + e, sc = 2 * (p * Kv4<D>::kGroups + el / 32);
-                const int kc = tile[kv4_key_byte(p, el >> 1)] >> (4 * (el & 1)) & 15;
-                const int vc = tile[Kv4<D>::kCodes + kv4_value_byte(p, el >> 1)] >> (4 * (el & 1)) & 15;
-                kx[e] = (kc - 8) * __half2float(*reinterpret_cast<const __half*>(tile + Kv4<D>::kKeyScales + sc));
-                vx[e] = (vc - 8) * __half2float(*reinterpret_cast<const __half*>(tile + Kv4<D>::kValueScales + sc));
+        for (int r = 0; r < 2; ++r) {
+            if constexpr (G == 4) {
+                const uint2 u = lds64(s + (g + 8 * r) * 8);
+                const float2 x = unpack_f16(u.x), y = unpack_f16(u.y);
+                out[r][0] = x.x, out[r][1] = x.y, out[r][2] = y.x, out[r][3] = y.y;
+            } else {
+                const float2 x = unpack_f16(*reinterpret_cast<const uint32_t*>(s + (g + 8 * r) * 4));
+                out[r][0] = x.x, out[r][1] = x.y;
             }
         }
+    }
+    // The value scales, and for both rows an exponent E with |scale| < 2^E for every group.
+    __device__ __forceinline__ static float2 load_value_scales(const uint8_t* s, int g, float (&out)[2][G]) {
+        float e[2];
 #pragma unroll
-        for (int h = 0; h < NREP; ++h) {
-            float s = 0.f;
+        for (int r = 0; r < 2; ++r) {
+            uint32_t top;
+            if constexpr (G == 4) {
+                const uint2 u = lds64(s + (g + 8 * r) * 8);
+                const float2 x = unpack_f16(u.x), y = unpack_f16(u.y);
+                out[r][0] = x.x, out[r][1] = x.y, out[r][2] = y.x, out[r][3] = y.y;
+                top = __vmaxu2(u.x & 0x7FFF7FFFu, u.y & 0x7FFF7FFFu);
+            } else {
+                const uint32_t u = *reinterpret_cast<const uint32_t*>(s + (g + 8 * r) * 4);
+                const float2 x = unpack_f16(u);
+                out[r][0] = x.x, out[r][1] = x.y;
+                top = u & 0x7FFF7FFFu;
+            }
+            top = max(top & 0xFFFFu, top >> 16);
+            e[r] = static_cast<float>(static_cast<int>(top >> 10) - 14);
+        }
+        return make_float2(e[0], e[1]);
+    }
+
+    // Sums over the warp's rows, to shared memory: o [NREP][D], m and l [NREP] (sums relative to 2^m).
+    __device__ __forceinline__ void finish(float* so, float* sm, float* sl, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        const int h0 = kWide ? 2 * t : 2 * (t & 1);  // this lane's columns are heads h0, h0 + 1
+        const bool mine = h0 < NREP && (kWide || t < 2);
+        l[0] = rows_sum(l[0]);
+        l[1] = rows_sum(l[1]);
 #pragma unroll
-            for (int e = 0; e < E; ++e) s = fmaf(kx[e], qs[h][lane * E + e], s);
-            s = warp_sum(s);
-            const float mn = fmaxf(m[h], s), c = m[h] == -INFINITY ? 0.f : expf(m[h] - mn), w = expf(s - mn);
-            m[h] = mn;
-            ls[h] = ls[h] * c + w;
+        for (int i = 0; i < G; ++i) {
+            ws[i][0] = 8.f * rows_sum(ws[i][0]);
+            ws[i][1] = 8.f * rows_sum(ws[i][1]);
+        }
 #pragma unroll
-            for (int e = 0; e < E; ++e) o[h][e] = fmaf(w, vx[e], o[h][e] * c);
+        for (int j = 0; j < KS; ++j) {
+            float y[4] = {o[j][0], o[j][1], o[j][2], o[j][3]};
+            if constexpr (!kWide) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) y[i] += __shfl_xor_sync(0xffffffffu, y[i], 2);
+            }
+            if (mine) {  // rows g and g + 8 are elements 16j + 2g, 16j + 2g + 1
+                const float w0 = ws[j / 2][0], w1 = ws[j / 2][1];
+                *reinterpret_cast<float2*>(so + h0 * D + 16 * j + 2 * g) =
+                    make_float2(fmaf(y[0], 16777216.f, -w0), fmaf(y[2], 1048576.f, -w0));
+                if (h0 + 1 < NREP)
+                    *reinterpret_cast<float2*>(so + (h0 + 1) * D + 16 * j + 2 * g) =
+                        make_float2(fmaf(y[1], 16777216.f, -w1), fmaf(y[3], 1048576.f, -w1));
+            }
+        }
+        if (mine && g == 0) {
+            sm[h0] = m[0] - 7.f, sl[h0] = l[0];
+            if (h0 + 1 < NREP) sm[h0 + 1] = m[1] - 7.f, sl[h0 + 1] = l[1];
         }
     }
-#pragma unroll
-    for (int h = 0; h < NREP; ++h) {
-        wm[warp][h] = m[h], wl[warp][h] = ls[h];
-#pragma unroll
-        for (int e = 0; e < E; ++e) wo[warp][h][lane * E + e] = o[h][e];
+};
+
+template <typename In, int D, int NREP>
+__global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kernel(const Kv4DecodeArgs a) {
+    using Sm = Kv4DecodeSmem<D, NREP>;
+    constexpr int L = D / 8, S = Sm::kStages, TB = Kv4<D>::kTileBytes, PF = kv4_part_floats(NREP, D);
+    extern __shared__ __align__(128) uint8_t smem[];
+    float* qs = reinterpret_cast<float*>(smem + Sm::kQ);
+    float* kn = reinterpret_cast<float*>(smem + Sm::kKn);
+    float* vn = reinterpret_cast<float*>(smem + Sm::kVn);
+    float2* cs = reinterpret_cast<float2*>(smem + Sm::kCs);
+    float* so = reinterpret_cast<float*>(smem + Sm::kO);
+    float* sm = reinterpret_cast<float*>(smem + Sm::kM);
+    float* sl = reinterpret_cast<float*>(smem + Sm::kL);
+    volatile int* abort = reinterpret_cast<volatile int*>(smem + Sm::kMisc);
+    int* last = reinterpret_cast<int*>(smem + Sm::kMisc + 4);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Sm::kBar) + warp * S;
+    uint8_t* ring = smem + Sm::kRing + size_t(warp) * S * TB;
+    if (lane == 0) {
+        for (int s = 0; s < S; ++s) mbar_init(&bars[s], 1);
+        fence_mbar_init();
     }
+    if (threadIdx.x == 0) *abort = 0;
     __syncthreads();
-    for (int i = threadIdx.x; i < NREP * D; i += 256) {
-        const int h = i / D;
-        float M = -INFINITY, s = 0.f, t = 0.f;
-        for (int w = 0; w < 8; ++w) M = fmaxf(M, wm[w][h]);
-        for (int w = 0; w < 8; ++w) {
-            const float c = wm[w][h] == -INFINITY ? 0.f : expf(wm[w][h] - M);
-            s = fmaf(wl[w][h], c, s);
-            t = fmaf(wo[w][h][i % D], c, t);
+    // Everything before touched only this block's shared memory; the previous kernel of the stream (which
+    // may have written the cache, the positions or the rows) has completed after this.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    const long long total = kv4_total(a, lane);
+    const int G = static_cast<int>(min(static_cast<long long>(gridDim.x), max(1ll, total / kKv4MinUnits)));
+    const int bx = blockIdx.x;
+    // Idle rows: zeros.
+    if (a.pos_rows) {
+        for (int r = bx; r < a.n_rows; r += gridDim.x) {
+            const int pos = a.pos_rows[r];
+            if (pos >= 0 && pos < a.n_context) continue;
+            if (pos >= 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = KERR_POSITION;
+            const float z[8] = {};
+            for (int u = threadIdx.x; u < a.q_heads * L; u += kKv4Threads)
+                store8(static_cast<In*>(a.out) + (static_cast<long long>(r) * a.q_heads * L + u) * 8, z);
+            for (int u = threadIdx.x; u < a.kv_heads * L; u += kKv4Threads) {
+                const long long at = (static_cast<long long>(r) * a.kv_heads * L + u) * 8;
+                if (a.k_rows) store_rows8(a.k_rows, a.rows_type, at, z);
+                if (a.v_rows) store_rows8(a.v_rows, a.rows_type, at, z);
+            }
         }
-        out[i] = KvTraits<In>::from_float(t / s);
     }
+    if (bx >= G) return;
+    const long long u0 = total * bx / G, u1 = total * (bx + 1) / G;
+    if (u0 >= u1) return;
+    const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
+    const long long head_bytes = a.tiles_per_head * TB;
+
+    // Two cursors walk the share's items: the copies', ahead, and the sums'.
+    struct Cursor {
+        int row, head, t, t1;  // next tile of this warp in the item's share, and its end
+        long long start, units, next;  // first unit and units of the row's head; first unit of the next head
+        Kv4Row r;
+    };
+    auto enter = [&](Cursor& c, long long u) {  // at unit u >= u0 of row c.row, whose heads start at c.start
+        c.r = kv4_row(a, kv4_pos(a, c.row));
+        c.units = c.r.nt + 1;
+        c.head = static_cast<int>((u - c.start) / c.units);
+        const long long h0 = c.start + c.head * c.units;
+        c.next = h0 + c.units;
+        c.t = static_cast<int>(u - h0) + warp;
+        c.t1 = static_cast<int>(min(static_cast<long long>(c.r.nt), u1 - h0));
+    };
+    auto advance = [&](Cursor& c) {  // to the next item of the share; false at its end
+        if (c.next >= u1) return false;
+        if (c.head + 1 == a.kv_heads) {
+            c.start = c.next;
+            do {
+                ++c.row;
+            } while (c.row + 1 < a.n_rows && kv4_units(a, kv4_pos(a, c.row)) == 0);
+        }
+        enter(c, c.next);
+        return true;
+    };
+    Cursor in;
+    in.row = kv4_find_row(a, u0, in.start, lane);
+    enter(in, u0);
+    Cursor at = in;
+    int issued = 0, taken = 0;
+    bool more = true;
+    auto fill = [&]() {  // requests tiles until the ring is full or the share's end
+        while (more && issued < taken + S) {
+            if (in.t >= in.t1) {
+                more = advance(in);
+                continue;
+            }
+            if (lane == 0) {
+                const int s = issued % S;
+                const uint8_t* src = a.tiles + (static_cast<long long>(in.row) * a.kv_heads + in.head) * head_bytes +
+                                     static_cast<long long>(kv4_tile_of(in.r, in.t)) * TB;
+                mbar_arrive_expect_tx(&bars[s], TB);
+                bulk_copy_g2s(ring + s * TB, src, TB, &bars[s]);
+            }
+            ++issued;
+            in.t += kKv4Warps;
+        }
+    };
+    fill();
+
+    Kv4Warp<D, NREP> acc;
+    long long seg0 = u0;  // first unit of the current item in this share
+    for (int seg = 0;; ++seg) {
+        const int pos = at.r.pos, g = at.head;
+        const long long item0 = at.next - at.units;
+        const bool own = at.next <= u1;  // the item's last unit, the token itself, is in this share
+        // Queries (and the token's own key and value) of the item.
+        for (int i = threadIdx.x; i < a.pairs; i += kKv4Threads) cs[i] = rope_turn(a.turns, i, pos, a.magnitude);
+        __syncthreads();
+        for (int job = warp; job < NREP + (own ? 2 : 0); job += kKv4Warps) {
+            const bool isq = job < NREP, isk = job == NREP;
+            const In* src = isq   ? static_cast<const In*>(a.q) + at.row * a.q_stride + (g * NREP + job) * D
+                            : isk ? static_cast<const In*>(a.k) + at.row * a.k_stride + g * D
+                                  : static_cast<const In*>(a.v) + at.row * a.v_stride + g * D;
+            float* dst = isq ? qs + job * D : isk ? kn : vn;
+            const bool rot = isq || isk;
+            float x[8];
+            kv4_head<In, D>(src, isq ? a.q_gamma : a.k_gamma, rot && a.norm, a.eps, cs, rot ? a.pairs : 0, a.layout, dst, x, lane);
+            if (!isq) {
+                uint32_t codes;
+                const __half d = kv4_quantize8(x, codes);
+                if (lane < L) {
+                    uint8_t* tile = a.tiles + (static_cast<long long>(at.row) * a.kv_heads + g) * head_bytes +
+                                    static_cast<long long>(pos / kKv4Tile) * TB;
+                    if (isk)
+                        kv4_store8<D, false>(tile, pos % kKv4Tile, lane, codes, d);
+                    else
+                        kv4_store8<D, true>(tile, pos % kKv4Tile, lane, codes, d);
+                    void* rows = isk ? a.k_rows : a.v_rows;
+                    if (rows) {
+                        float y[8];
+                        kv4_values8(codes, d, y);
+                        store_rows8(rows, a.rows_type, (static_cast<long long>(at.row) * a.kv_heads + g) * D + lane * 8, y);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] *= a.scale_log2;
+            }
+            if (lane < L) store8(dst + lane * 8, x);
+        }
+        __syncthreads();
+        acc.start(qs, lane);
+        bool ok = true;
+        for (; at.t < at.t1; at.t += kKv4Warps) {
+            const int s = taken % S;
+            ok = mbar_wait_bounded(&bars[s], (taken / S) & 1, deadline, abort);
+            if (!__all_sync(0xffffffffu, ok)) {
+                if (lane == 0) {
+                    *abort = 1;
+                    *reinterpret_cast<volatile int*>(a.err) = KERR_TIMEOUT_FULL;
+                }
+                ok = false;
+                break;
+            }
+            acc.tile(ring + s * TB, at.r, kv4_tile_of(at.r, at.t) * kKv4Tile, lane);
+            __syncwarp();
+            ++taken;
+            fill();
+        }
+        acc.finish(so + warp * NREP * D, sm + warp * NREP, sl + warp * NREP, lane);
+        if (own)  // the token itself: one key whose weight is 1 relative to its own score
+            for (int h = warp; h < NREP; h += kKv4Warps) {
+                float x = 0.f;
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i) x = fmaf(qs[h * D + lane + 32 * i], kn[lane + 32 * i], x);
+                x = warp_sum(x);
+                if (lane == 0) sm[kKv4Warps * NREP + h] = x, sl[kKv4Warps * NREP + h] = 1.f;
+            }
+        __syncthreads();
+        if (*abort) break;  // raised before the barrier: every thread sees it
+        // Join the warps.
+        const int parts = own ? kKv4Warps + 1 : kKv4Warps;
+        const bool whole = own && seg0 == item0;  // no other block has a part of this item
+        const long long item = static_cast<long long>(at.row) * a.kv_heads + g;
+        In* out = static_cast<In*>(a.out) + item * NREP * D;
+        float* mine = a.parts + (static_cast<long long>(bx) * 2 + (seg ? 1 : 0)) * PF;
+        for (int i = threadIdx.x; i < NREP * D; i += kKv4Threads) {
+            const int h = i / D;
+            float M = sm[h];
+            for (int w = 1; w < parts; ++w) M = fmaxf(M, sm[w * NREP + h]);
+            float lsum = 0.f, osum = 0.f;
+            for (int w = 0; w < kKv4Warps; ++w) {
+                const float f = ex2(sm[w * NREP + h] - M);
+                lsum = fmaf(sl[w * NREP + h], f, lsum);
+                osum = fmaf(so[w * NREP * D + i], f, osum);
+            }
+            if (own) {
+                const float f = ex2(sm[kKv4Warps * NREP + h] - M);
+                lsum += f;
+                osum = fmaf(vn[i % D], f, osum);
+            }
+            if (whole) {
+                out[i] = KvTraits<In>::from_float(osum / lsum);
+            } else {
+                mine[i] = osum;
+                if (i % D == 0) mine[NREP * D + h] = M, mine[NREP * D + NREP + h] = lsum;
+            }
+        }
+        if (!whole) {
+            __threadfence();
+            __syncthreads();
+            // Blocks b0..b1 have parts of the item: those whose shares meet [item0, at.next).
+            const int b0 = static_cast<int>((item0 * G + G - 1) / total), b1 = static_cast<int>(((at.next - 1) * G + G - 1) / total);
+            // (the share of block b is [total * b / G, total * (b + 1) / G), rounded down)
+            int f = b0, e = b1;
+            while (f > 0 && total * f / G > item0) --f;
+            while (f + 1 < G && total * (f + 1) / G <= item0) ++f;
+            while (e > 0 && total * e / G > at.next - 1) --e;
+            while (e + 1 < G && total * (e + 1) / G <= at.next - 1) ++e;
+            if (threadIdx.x == 0) {
+                const int n = atomicAdd(a.tickets + item, 1);
+                *last = n == e - f;
+                if (*last) a.tickets[item] = 0;
+            }
+            __syncthreads();
+            if (*last) {
+                __threadfence();
+                const int n = e - f + 1;
+                // Block f's part lies in its second slot when the item began inside its share.
+                const float* p0 = a.parts + (static_cast<long long>(f) * 2 + (total * f / G < item0 ? 1 : 0)) * PF;
+                auto part = [&](int i) { return i ? a.parts + static_cast<long long>(f + i) * 2 * PF : p0; };
+                for (int i = threadIdx.x; i < NREP * D; i += kKv4Threads) {
+                    const int h = i / D;
+                    float M = -INFINITY, lsum = 0.f, osum = 0.f;
+                    for (int w = 0; w < n; ++w) M = fmaxf(M, __ldcg(part(w) + NREP * D + h));
+                    for (int w = 0; w < n; ++w) {
+                        const float* p = part(w);
+                        const float fw = ex2(__ldcg(p + NREP * D + h) - M);
+                        lsum = fmaf(__ldcg(p + NREP * D + NREP + h), fw, lsum);
+                        osum = fmaf(__ldcg(p + i), fw, osum);
+                    }
+                    out[i] = KvTraits<In>::from_float(osum / lsum);
+                }
+            }
+        }
+        seg0 = at.next;
+        if (!advance(at)) break;
+        __syncthreads();  // the next item overwrites what this one's join read
+    }
+    // After a wait that gave up, the copies in flight land before the block ends.
+    for (; taken < issued; ++taken)
+        while (!mbar_try_wait(&bars[taken % S], (taken / S) & 1) && globaltimer_ns() < deadline + kWaitLimitNs / 2) {
+        }
 }
 
 }  // namespace lg

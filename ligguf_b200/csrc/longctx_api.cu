@@ -134,6 +134,9 @@ int launch_rope_rows_any(lg::RopeRowsArgs& a, const ligguf_rope_cfg& r, int in_t
     }
 }
 
+// Blocks of the decode kernel resident per SM (its __launch_bounds__ minimum).
+int kv4_blocks_per_sm(int nrep) { return nrep > 4 ? 1 : 2; }
+
 int make_err_word(int** h_err, int** d_err) {
     if (cudaHostAlloc(reinterpret_cast<void**>(h_err), 64, cudaHostAllocMapped) != cudaSuccess)
         return fail(LIGGUF_ATTN_ENOMEM, "mapped error word");
@@ -158,6 +161,9 @@ struct ligguf_kv4 {
     double* turns = nullptr;
     float* gammas = nullptr;          // [n_layers][2][head_dim]
     unsigned char* norm_set = nullptr;  // [n_layers], host
+    float* parts = nullptr;  // decode: partial results of items that several blocks share
+    int* tickets = nullptr;  // decode: [n_seqs * n_kv_heads] blocks done with such an item; zero between calls
+    int num_sms = 0;
     int *h_err = nullptr, *d_err = nullptr;
     uint8_t* seq_tiles(int layer, int seq) const {
         return tiles + (static_cast<size_t>(layer) * cfg.n_seqs + seq) * cfg.n_kv_heads * tiles_per_head * tile_bytes;
@@ -182,21 +188,45 @@ int kv4_check(const ligguf_kv4* h, int layer, int seq, int n_seqs, int pos0, int
     return LIGGUF_ATTN_OK;
 }
 
-template <typename In, int D>
-int launch_kv4_decode(const lg::Kv4DecodeArgs& a, int nrep, cudaStream_t st) {
-    const dim3 grid(a.kv_heads, a.n_rows);
-    switch (nrep) {
-        case 1: lg::kv4_decode_kernel<In, D, 1><<<grid, 256, 0, st>>>(a); break;
-        case 2: lg::kv4_decode_kernel<In, D, 2><<<grid, 256, 0, st>>>(a); break;
-        case 4: lg::kv4_decode_kernel<In, D, 4><<<grid, 256, 0, st>>>(a); break;
-        default: lg::kv4_decode_kernel<In, D, 8><<<grid, 256, 0, st>>>(a); break;
+template <typename In, int D, int NREP>
+int launch_kv4_decode(const ligguf_kv4* h, const lg::Kv4DecodeArgs& a, cudaStream_t st) {
+    using Sm = lg::Kv4DecodeSmem<D, NREP>;
+    auto kern = lg::kv4_decode_kernel<In, D, NREP>;
+    static bool attr_done[64] = {};
+    const int device = h->cfg.device;
+    if (device >= 64 || !attr_done[device]) {
+        LG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Sm::kTotal)));
+        if (device < 64) attr_done[device] = true;
     }
-    LG_CUDA(cudaGetLastError());
+    // As many blocks as fit at once, fewer when the longest visible contexts do not fill them.
+    const long long keys = std::min<long long>(h->cfg.n_context, a.window ? 2ll * lg::kKv4Tile + a.window + a.sinks : INT32_MAX);
+    const long long units = (keys / lg::kKv4Tile + 2) * a.kv_heads * a.n_rows;
+    const int slots = h->num_sms * kv4_blocks_per_sm(NREP);
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3(static_cast<unsigned>(std::min<long long>(slots, std::max<long long>(1, units / lg::kKv4MinUnits))));
+    lc.blockDim = dim3(lg::kKv4Threads);
+    lc.dynamicSmemBytes = Sm::kTotal;
+    lc.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = attr;
+    lc.numAttrs = 1;
+    LG_CUDA(cudaLaunchKernelEx(&lc, kern, a));
     return LIGGUF_ATTN_OK;
 }
+template <typename In, int D>
+int launch_kv4_decode_n(const ligguf_kv4* h, const lg::Kv4DecodeArgs& a, cudaStream_t st) {
+    switch (h->nrep) {
+        case 1: return launch_kv4_decode<In, D, 1>(h, a, st);
+        case 2: return launch_kv4_decode<In, D, 2>(h, a, st);
+        case 4: return launch_kv4_decode<In, D, 4>(h, a, st);
+        default: return launch_kv4_decode<In, D, 8>(h, a, st);
+    }
+}
 template <typename In>
-int launch_kv4_decode_d(const lg::Kv4DecodeArgs& a, int D, int nrep, cudaStream_t st) {
-    return D == 64 ? launch_kv4_decode<In, 64>(a, nrep, st) : launch_kv4_decode<In, 128>(a, nrep, st);
+int launch_kv4_decode_d(const ligguf_kv4* h, const lg::Kv4DecodeArgs& a, cudaStream_t st) {
+    return h->cfg.rope.head_dim == 64 ? launch_kv4_decode_n<In, 64>(h, a, st) : launch_kv4_decode_n<In, 128>(h, a, st);
 }
 
 lg::Kv4IoArgs kv4_io(const ligguf_kv4* h, int layer, int seq, int n_seqs, int pos0, int n, void* k, void* v) {
@@ -340,6 +370,8 @@ int ligguf_cuda_kv4_free(ligguf_kv4* h) {
     cudaFree(h->tiles);
     cudaFree(h->turns);
     cudaFree(h->gammas);
+    cudaFree(h->parts);
+    cudaFree(h->tickets);
     if (h->h_err) cudaFreeHost(h->h_err);
     delete[] h->norm_set;
     delete h;
@@ -394,10 +426,16 @@ int ligguf_cuda_kv4_init(const ligguf_kv4_cfg* cfg, ligguf_kv4** out) {
         (void)cudaGetLastError();
         return bail(fail(LIGGUF_ATTN_ENOMEM, "4-bit cache of %zu bytes does not fit", bytes));
     }
-    if (cudaMalloc(&h->gammas, gbytes) != cudaSuccess) {
+    if (cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, c.device) != cudaSuccess)
+        return bail(fail(LIGGUF_ATTN_ECUDA, "cudaDeviceGetAttribute failed"));
+    const size_t part_bytes = size_t(h->num_sms) * kv4_blocks_per_sm(nrep) * 2 * lg::kv4_part_floats(nrep, D) * sizeof(float);
+    const size_t ticket_bytes = size_t(c.n_seqs) * c.n_kv_heads * sizeof(int);
+    if (cudaMalloc(&h->gammas, gbytes) != cudaSuccess || cudaMalloc(&h->parts, part_bytes) != cudaSuccess ||
+        cudaMalloc(&h->tickets, ticket_bytes) != cudaSuccess) {
         (void)cudaGetLastError();
-        return bail(fail(LIGGUF_ATTN_ENOMEM, "norm weights"));
+        return bail(fail(LIGGUF_ATTN_ENOMEM, "handle buffers"));
     }
+    if (cudaMemset(h->tickets, 0, ticket_bytes) != cudaSuccess) return bail(fail(LIGGUF_ATTN_ECUDA, "cudaMemset of the tickets failed"));
     // Zeroed like the engine's cache: unwritten positions are zeros, not whatever lay there.
     if (cudaMemset(h->tiles, 0, bytes) != cudaSuccess) return bail(fail(LIGGUF_ATTN_ECUDA, "cudaMemset of the cache failed"));
     if ((rc = make_turns(c.rope, &h->turns)) || (rc = make_err_word(&h->h_err, &h->d_err))) return bail(rc);
@@ -497,17 +535,19 @@ int ligguf_cuda_kv4_decode_async(ligguf_kv4* h, int layer, int n_rows, int pos, 
     a.rows_type = c.rows_type;
     a.eps = c.rms_epsilon;
     a.magnitude = c.rope.magnitude > 0.f ? c.rope.magnitude : 1.f;
-    a.scale = c.scale;
+    a.scale_log2 = c.scale * 1.4426950408889634f;
     a.window = c.window;
     a.sinks = c.sinks;
     a.tiles = h->seq_tiles(layer, 0);
     a.tiles_per_head = h->tiles_per_head;
+    a.parts = h->parts;
+    a.tickets = h->tickets;
     a.err = h->d_err;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (c.in_type) {
-        case LIGGUF_KV_F32: return launch_kv4_decode_d<float>(a, D, h->nrep, st);
-        case LIGGUF_KV_F16: return launch_kv4_decode_d<__half>(a, D, h->nrep, st);
-        default: return launch_kv4_decode_d<__nv_bfloat16>(a, D, h->nrep, st);
+        case LIGGUF_KV_F32: return launch_kv4_decode_d<float>(h, a, st);
+        case LIGGUF_KV_F16: return launch_kv4_decode_d<__half>(h, a, st);
+        default: return launch_kv4_decode_d<__nv_bfloat16>(h, a, st);
     }
 }
 
@@ -558,7 +598,10 @@ int ligguf_cuda_kv4_status(ligguf_kv4* h, void* stream) {
     const int code = *reinterpret_cast<volatile int*>(h->h_err);
     *reinterpret_cast<volatile int*>(h->h_err) = 0;
     if (code == lg::KERR_POSITION) return fail(LIGGUF_ATTN_EINVAL, "a decode row's position is beyond n_context %d", h->cfg.n_context);
-    if (code) return fail(LIGGUF_ATTN_ETIMEDOUT, "a bounded in-kernel wait gave up (kernel error code %d)", code);
+    if (code) {  // blocks that gave up left tickets behind
+        LG_CUDA(cudaMemset(h->tickets, 0, size_t(h->cfg.n_seqs) * h->cfg.n_kv_heads * sizeof(int)));
+        return fail(LIGGUF_ATTN_ETIMEDOUT, "a bounded in-kernel wait gave up (kernel error code %d)", code);
+    }
     return LIGGUF_ATTN_OK;
 }
 
