@@ -14,19 +14,22 @@
 //   - S^T = K Q^T: 16 positions x 8 columns.  The key scales multiply the fp32 sums of their 32 elements.
 //   - Queries and weights are split into two halves each, hi + lo, which together hold 22 bits, so the
 //     results are those of fp32 arithmetic.  Up to four query heads a KV head share one product: columns
-//     0-3 are the hi parts of the heads, 4-7 the lo parts, which cost nothing then.  With eight heads the
-//     lo parts are a second product into the same sums.
+//     0-3 are the hi parts of the heads, 4-7 the lo parts, which cost nothing then.  The two parts of a
+//     score lie two lanes apart, so a warp takes tiles in pairs: one exchange leaves the lanes of the hi
+//     columns with the first tile's scores and those of the lo columns with the second's, and no lane
+//     does another's softmax again.  With eight heads the lo parts are a second product into the same
+//     sums, and every lane has heads of its own.
 //   - O^T += V^T W: the value scales are multiplied into the weights, one B operand for each 32 elements.
 //     The weights go from the sums' layout to the operand's by transposing 8x8 fragments (movmatrix).
 //   - Weights carry value scales of any size, so the running maximum is that of x_j + (exponent of the
 //     largest scale of row j): |weight * scale| stays in [0, 2^15] of fp16's range whatever the scales.
 //     It is only moved when a row exceeds it by 2^8, a vote of the warp per tile.
 //
-// The work is one list: (row, KV head) items, each its visible tiles and one unit more for the token
-// itself, cut into equal contiguous shares of as many blocks as fit at once, whatever the lengths of the
-// sequences; the cut is computed by every block from the positions, which may be in device memory.  In a
-// share, the 8 warps take tiles in turn, each with its own ring of bulk copies and its own running sums,
-// which the block joins per item.  Items that several blocks share are joined by the last of them to
+// The work is one list: (row, KV head) items, each some units for its start and end, its visible tiles, and
+// one unit for the token itself, cut into equal contiguous shares of as many blocks as fit at once, whatever
+// the lengths of the sequences; the cut is computed by every block from the positions, which may be in
+// device memory.  In a share, the 8 warps take pairs of tiles in turn, each with its own ring of bulk copies
+// and its own running sums, which the block joins per item.  Items that several blocks share are joined by the last of them to
 // finish, in the order of the blocks, so results repeat bit for bit.
 #pragma once
 
@@ -58,16 +61,19 @@ enum : int { KERR_POSITION = 16 };
 
 constexpr int kKv4Warps = 8;
 constexpr int kKv4Threads = 32 * kKv4Warps;
-constexpr int kKv4MinUnits = kKv4Warps;  // tiles a block has at least: fewer blocks share a short context
+constexpr int kKv4MinUnits = 2 * kKv4Warps;  // units a block has at least: fewer blocks share a short context
+// Units that an item counts beside its tiles and its token: what a block spends on entering and joining an
+// item, in tiles.
+constexpr int kKv4ItemUnits = 24;
 
 // Floats of one partial result: o [NREP][D], m [NREP], l [NREP].
 __host__ __device__ constexpr int kv4_part_floats(int nrep, int dim) { return nrep * (dim + 2); }
 
 template <int D, int NREP>
 struct Kv4DecodeSmem {
-    static constexpr int kStages = D == 128 ? 4 : 8;
+    static constexpr int kStages = D == 128 ? 2 : 4;  // pairs of tiles a warp has in flight
     static constexpr size_t kRing = 0;
-    static constexpr size_t kQ = kRing + size_t(kKv4Warps) * kStages * Kv4<D>::kTileBytes;
+    static constexpr size_t kQ = kRing + size_t(kKv4Warps) * kStages * 2 * Kv4<D>::kTileBytes;
     static constexpr size_t kKn = kQ + NREP * D * 4;
     static constexpr size_t kVn = kKn + D * 4;
     static constexpr size_t kCs = kVn + D * 4;
@@ -95,68 +101,79 @@ __device__ __forceinline__ Kv4Row kv4_row(const Kv4DecodeArgs& a, int pos) {
     return r;
 }
 __device__ __forceinline__ int kv4_tile_of(const Kv4Row& r, int i) { return i < r.ns ? i : r.tw + (i - r.ns); }
-// Units of one head of a row: its tiles and the token itself; none for an idle row.
-__device__ __forceinline__ long long kv4_units(const Kv4DecodeArgs& a, int pos) {
-    return pos < 0 || pos >= a.n_context ? 0 : kv4_row(a, pos).nt + 1;
-}
-__device__ __forceinline__ int kv4_pos(const Kv4DecodeArgs& a, int r) { return a.pos_rows ? __ldg(a.pos_rows + r) : a.pos; }
-
-// The row (returned) whose units hold unit u of the whole list, and the first of its units; n_rows if none.
-// Warp-collective.
-__device__ __forceinline__ int kv4_find_row(const Kv4DecodeArgs& a, long long u, long long& start, int lane) {
-    if (!a.pos_rows) {
-        const long long per = kv4_units(a, a.pos) * a.kv_heads;
-        const int r = per ? static_cast<int>(u / per) : a.n_rows;
-        start = r * per;
-        return r;
-    }
-    long long before = 0;
-    for (int r0 = 0; r0 < a.n_rows; r0 += 32) {
-        const long long mine = r0 + lane < a.n_rows ? kv4_units(a, a.pos_rows[r0 + lane]) * a.kv_heads : 0;
-        long long upto = mine;  // inclusive scan
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long x = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += x;
-        }
-        const unsigned past = __ballot_sync(0xffffffffu, before + upto > u);
-        if (past) {
-            const int w = __ffs(past) - 1;
-            start = before + __shfl_sync(0xffffffffu, upto - mine, w);
-            return r0 + w;
-        }
-        before += __shfl_sync(0xffffffffu, upto, 31);
-    }
-    start = before;
-    return a.n_rows;
-}
-__device__ __forceinline__ long long kv4_total(const Kv4DecodeArgs& a, int lane) {
-    if (!a.pos_rows) return kv4_units(a, a.pos) * a.kv_heads * a.n_rows;
-    long long n = 0;
-    for (int r = lane; r < a.n_rows; r += 32) n += kv4_units(a, a.pos_rows[r]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-    return n * a.kv_heads;
+// Units of one head of a row; none for an idle row.  (The launcher keeps the sum of all below 2^31.)
+__device__ __forceinline__ int kv4_units(const Kv4DecodeArgs& a, int pos) {
+    return pos < 0 || pos >= a.n_context ? 0 : kKv4ItemUnits + kv4_row(a, pos).nt + 1;
 }
 
-// One head (8 elements a lane, D/8 lanes, the other lanes the same again): norm and rotation; `dst`
-// (shared, D floats) carries the exchange and gets the result.
-template <typename In, int D>
-__device__ __forceinline__ void kv4_head(const In* src, const float* gamma, bool norm, float eps, const float2* cs,
-                                         int pairs, int layout, float* dst, float (&x)[8], int lane) {
+// The positions of a call.  Up to 32 rows: one load, a row a lane.
+struct Kv4Positions {
+    int mine;  // row `lane`, when there are at most 32
+    __device__ __forceinline__ void load(const Kv4DecodeArgs& a, int lane) {
+        mine = -1;
+        if (a.pos_rows && a.n_rows <= 32 && lane < a.n_rows) mine = a.pos_rows[lane];
+    }
+    // Warp-uniform r.
+    __device__ __forceinline__ int at(const Kv4DecodeArgs& a, int r) const {
+        if (!a.pos_rows) return a.pos;
+        if (a.n_rows <= 32) return __shfl_sync(0xffffffffu, mine, r);
+        return a.pos_rows[r];
+    }
+    __device__ __forceinline__ int lane_at(const Kv4DecodeArgs& a, int r0, int lane) const {
+        if (a.n_rows <= 32) return mine;
+        return r0 + lane < a.n_rows ? a.pos_rows[r0 + lane] : -1;
+    }
+    // All units (warp-collective).
+    __device__ __forceinline__ int total(const Kv4DecodeArgs& a, int lane) const {
+        if (!a.pos_rows) return kv4_units(a, a.pos) * a.kv_heads * a.n_rows;
+        int n = 0;
+        for (int r0 = 0; r0 < a.n_rows; r0 += 32) n += kv4_units(a, lane_at(a, r0, lane));
+        return __reduce_add_sync(0xffffffffu, n) * a.kv_heads;
+    }
+    // The row that holds unit u of the list, and the first of its units (warp-collective).
+    __device__ __forceinline__ int find(const Kv4DecodeArgs& a, int u, int& start, int lane) const {
+        if (!a.pos_rows) {
+            const int per = kv4_units(a, a.pos) * a.kv_heads;
+            start = u / per * per;
+            return u / per;
+        }
+        int before = 0;
+        for (int r0 = 0; r0 < a.n_rows; r0 += 32) {
+            const int own = kv4_units(a, lane_at(a, r0, lane)) * a.kv_heads;
+            int upto = own;  // inclusive scan
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += x;
+            }
+            const unsigned past = __ballot_sync(0xffffffffu, before + upto > u);
+            if (past) {
+                const int w = __ffs(past) - 1;
+                start = before + __shfl_sync(0xffffffffu, upto - own, w);
+                return r0 + w;
+            }
+            before += __shfl_sync(0xffffffffu, upto, 31);
+        }
+        start = before;
+        return a.n_rows - 1;
+    }
+};
+
+// One head, 8 elements a lane (D/8 lanes, the other lanes the same again): norm and rotation of x; `dst`
+// (shared, D floats) carries the exchange.
+template <int D>
+__device__ __forceinline__ void kv4_head(float (&x)[8], const float (&gamma)[8], bool norm, float eps, const float2* cs,
+                                         int pairs, int layout, float* dst, int lane) {
     constexpr int L = D / 8;
     const int l = lane % L;
-    load8(src + l * 8, x);
     if (norm) {
-        float g[8];
-        load8(gamma + l * 8, g);
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
         ss = head_sum<L>(ss);
         const float rs = 1.0f / sqrtf(ss / static_cast<float>(D) + eps);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (x[i] * rs) * g[i];
+        for (int i = 0; i < 8; ++i) x[i] = (x[i] * rs) * gamma[i];
     }
     if (layout == LIGGUF_ROPE_ADJACENT) {
 #pragma unroll
@@ -167,7 +184,7 @@ __device__ __forceinline__ void kv4_head(const In* src, const float* gamma, bool
                 x[2 * i] = x0 * w.x - x1 * w.y;
                 x[2 * i + 1] = x0 * w.y + x1 * w.x;
             }
-    } else {
+    } else if (pairs) {
         if (lane < L) store8(dst + l * 8, x);
         __syncwarp();
 #pragma unroll
@@ -223,10 +240,11 @@ __device__ __forceinline__ uint2 lds64(const void* p) {
     return r;
 }
 
-// Sum over the 8 lanes (row groups) that share a fragment's column pair.
+// Sum over the lanes whose heads are the same: the 8 row groups, and (kWide: not) the pair's two tiles.
+template <bool kWide>
 __device__ __forceinline__ float rows_sum(float v) {
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int o = kWide ? 4 : 2; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
@@ -236,7 +254,7 @@ struct Kv4Warp {
     static constexpr bool kWide = NREP > 4;  // hi and lo parts as two products
     static constexpr int KS = D / 16, G = D / 32;
     uint32_t b[kWide ? 2 : 1][KS][2];  // queries, as B operands
-    float c[kWide ? 2 : 1][G][2];      // -8 * sum of a group's queries, of this lane's columns
+    float c[G][2];                     // -8 * sum of a group's queries, of this lane's columns
     float sx[2];                       // scales of the scores of this lane's two heads
     float m[2], l[2], ws[G][2];        // running maxima, sums of weights and of weights * value scales
     float o[KS][4];
@@ -286,16 +304,14 @@ struct Kv4Warp {
         }
         // The sums of a column lie in the four lanes of its row group; this lane's columns are 2t, 2t+1.
 #pragma unroll
-        for (int p = 0; p < (kWide ? 2 : 1); ++p)
-#pragma unroll
-            for (int i = 0; i < G; ++i) {
-                float s = kWide ? sum[p][i] : (is_lo ? sum[1][i] : sum[0][i]);
-                s += __shfl_xor_sync(0xffffffffu, s, 1);
-                s += __shfl_xor_sync(0xffffffffu, s, 2);
-                s *= -8.f / 16777216.f;
-                c[p][i][0] = __shfl_sync(0xffffffffu, s, 8 * t);
-                c[p][i][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
-            }
+        for (int i = 0; i < G; ++i) {
+            float v = kWide ? sum[0][i] + sum[1][i] : (is_lo ? sum[1][i] : sum[0][i]);
+            v += __shfl_xor_sync(0xffffffffu, v, 1);
+            v += __shfl_xor_sync(0xffffffffu, v, 2);
+            v *= -8.f / 16777216.f;
+            c[i][0] = __shfl_sync(0xffffffffu, v, 8 * t);
+            c[i][1] = __shfl_sync(0xffffffffu, v, 8 * t + 4);
+        }
         const float down = __int_as_float((127 + e + 14) << 23);  // 2^(e - 10) * 2^24
         sx[0] = __shfl_sync(0xffffffffu, down, 8 * t);
         sx[1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
@@ -307,50 +323,46 @@ struct Kv4Warp {
         for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     }
 
-    // One tile in shared memory; positions k0 + row.
-    __device__ __forceinline__ void tile(const uint8_t* tp, const Kv4Row& r, int k0, int lane) {
-        const int g = lane >> 2;
-        // Scores of positions g (x[0], x[1]) and g + 8 (x[2], x[3]) with this lane's columns.
-        float x[4] = {0.f, 0.f, 0.f, 0.f};
-        {
-            float ks[2][G];
-            load_scales(tp + Kv4<D>::kKeyScales, g, ks);
+    // Raw scores of a tile's positions g (x[0], x[1]) and g + 8 (x[2], x[3]) with this lane's columns.
+    __device__ __forceinline__ void scores(const uint8_t* tp, int lane, float (&x)[4]) const {
+        float ks[2][G];
+        load_scales(tp + Kv4<D>::kKeyScales, lane >> 2, ks);
+        x[0] = x[1] = x[2] = x[3] = 0.f;
 #pragma unroll
-            for (int ch = 0; ch < D / 64; ++ch) {
-                const uint4 w4 = lds128(tp + ch * 512 + lane * 16);
-                const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+        for (int ch = 0; ch < D / 64; ++ch) {
+            const uint4 w4 = lds128(tp + ch * 512 + lane * 16);
+            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-                for (int gr = 0; gr < 2; ++gr) {
-                    const int i = ch * 2 + gr;
-                    float s[4] = {c[0][i][0], c[0][i][1], c[0][i][0], c[0][i][1]};
-                    if constexpr (kWide) s[0] += c[1][i][0], s[1] += c[1][i][1], s[2] += c[1][i][0], s[3] += c[1][i][1];
+            for (int gr = 0; gr < 2; ++gr) {
+                const int i = ch * 2 + gr;
+                float s[4] = {c[i][0], c[i][1], c[i][0], c[i][1]};
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const int j = 2 * i + u;
-                        const uint32_t lo = w[2 * gr + u], hi = lo >> 8;
-                        const uint32_t a0 = lo & 0x000F000Fu, a2 = lo & 0x00F000F0u, a1 = hi & 0x000F000Fu, a3 = hi & 0x00F000F0u;
-                        mma_f16(s, a0, a1, a2, a3, b[0][j][0], b[0][j][1], s[0], s[1], s[2], s[3]);
-                        if constexpr (kWide) mma_f16(s, a0, a1, a2, a3, b[1][j][0], b[1][j][1], s[0], s[1], s[2], s[3]);
-                    }
-                    x[0] = fmaf(s[0], ks[0][i], x[0]);
-                    x[1] = fmaf(s[1], ks[0][i], x[1]);
-                    x[2] = fmaf(s[2], ks[1][i], x[2]);
-                    x[3] = fmaf(s[3], ks[1][i], x[3]);
+                for (int u = 0; u < 2; ++u) {
+                    const int j = 2 * i + u;
+                    const uint32_t lo = w[2 * gr + u], hi = lo >> 8;
+                    const uint32_t a0 = lo & 0x000F000Fu, a2 = lo & 0x00F000F0u, a1 = hi & 0x000F000Fu, a3 = hi & 0x00F000F0u;
+                    mma_f16(s, a0, a1, a2, a3, b[0][j][0], b[0][j][1], s[0], s[1], s[2], s[3]);
+                    if constexpr (kWide) mma_f16(s, a0, a1, a2, a3, b[1][j][0], b[1][j][1], s[0], s[1], s[2], s[3]);
                 }
+                x[0] = fmaf(s[0], ks[0][i], x[0]);
+                x[1] = fmaf(s[1], ks[0][i], x[1]);
+                x[2] = fmaf(s[2], ks[1][i], x[2]);
+                x[3] = fmaf(s[3], ks[1][i], x[3]);
             }
         }
-        if constexpr (!kWide) {  // hi and lo columns of a head lie two lanes apart; both get the sum
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], 2);
-        }
+    }
+    // Softmax weights of a tile's positions k0 + g, k0 + g + 8 from their raw scores; vs: their value scales.
+    // masked: some position of the tile (or of the pair's other tile) is unseen.
+    __device__ __forceinline__ void weights(const uint8_t* tp, const Kv4Row& r, int k0, bool masked, bool there, int lane,
+                                            float (&x)[4], float (&p)[4], float (&vs)[2][G]) {
+        const int g = lane >> 2;
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] *= sx[i & 1];
-        float vs[2][G];
         const float2 ex = load_value_scales(tp + Kv4<D>::kValueScales, g, vs);
-        if (k0 + kKv4Tile > r.pos || k0 < r.first) {
+        if (masked) {
             const int j0 = k0 + g, j1 = j0 + 8;
-            const bool s0 = j0 < r.pos && (j0 >= r.first || j0 < r.sinks);
-            const bool s1 = j1 < r.pos && (j1 >= r.first || j1 < r.sinks);
+            const bool s0 = there && j0 < r.pos && (j0 >= r.first || j0 < r.sinks);
+            const bool s1 = there && j1 < r.pos && (j1 >= r.first || j1 < r.sinks);
             if (!s0) x[0] = x[1] = -INFINITY;
             if (!s1) x[2] = x[3] = -INFINITY;
 #pragma unroll
@@ -359,53 +371,103 @@ struct Kv4Warp {
                 if (!s1) vs[1][i] = 0.f;
             }
         }
-        const float y[4] = {x[0] + ex.x, x[1] + ex.x, x[2] + ex.y, x[3] + ex.y};
-        const float t0 = fmaxf(y[0], y[2]), t1 = fmaxf(y[1], y[3]);
+        const float t0 = fmaxf(x[0] + ex.x, x[2] + ex.y), t1 = fmaxf(x[1] + ex.x, x[3] + ex.y);
         if (__any_sync(0xffffffffu, t0 > m[0] + 8.f || t1 > m[1] + 8.f)) move_max(t0, t1);
-        float p[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = ex2(x[i] - m[i & 1] + 7.f);
+        const float m0 = m[0] - 7.f, m1 = m[1] - 7.f;
+        p[0] = ex2(x[0] - m0), p[1] = ex2(x[1] - m1), p[2] = ex2(x[2] - m0), p[3] = ex2(x[3] - m1);
         l[0] += p[0] + p[2];
         l[1] += p[1] + p[3];
-        const float lo_lane = (lane & 2) ? -1.f : 0.f;
+    }
+    // O += V^T W for one word of the value codes (16 elements of the head).
+    __device__ __forceinline__ void values(uint32_t lo, int j, uint32_t b0, uint32_t b1) {
+        const uint32_t hi = lo >> 8;
+        mma_f16(o[j], lo & 0x000F000Fu, lo & 0x00F000F0u, hi & 0x000F000Fu, hi & 0x00F000F0u, b0, b1, o[j][0], o[j][1], o[j][2],
+                o[j][3]);
+    }
+    __device__ __forceinline__ static bool edge(const Kv4Row& r, int k0) { return k0 + kKv4Tile > r.pos || k0 < r.first; }
+
+    // Two tiles in shared memory, of positions k0.. and k1.. (k1 < 0: only the first is there).
+    __device__ __forceinline__ void pair(const uint8_t* tp, const Kv4Row& r, int k0, int k1, int lane) {
+        constexpr int TB = Kv4<D>::kTileBytes;
+        if constexpr (kWide) {
+#pragma unroll 1
+            for (int n = 0; n < 2; ++n, tp += TB, k0 = k1) {
+                if (k0 < 0) return;
+                float x[4], p[4], vs[2][G];
+                scores(tp, lane, x);
+                weights(tp, r, k0, edge(r, k0), true, lane, x, p, vs);
 #pragma unroll
-        for (int ch = 0; ch < D / 64; ++ch) {
-            const uint4 w4 = lds128(tp + Kv4<D>::kCodes + ch * 512 + lane * 16);
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+                for (int ch = 0; ch < D / 64; ++ch) {
+                    const uint4 w4 = lds128(tp + Kv4<D>::kCodes + ch * 512 + lane * 16);
+                    const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
 #pragma unroll
-            for (int gr = 0; gr < 2; ++gr) {
-                const int i = ch * 2 + gr;
-                const float v0 = p[0] * vs[0][i], v1 = p[1] * vs[0][i], v2 = p[2] * vs[1][i], v3 = p[3] * vs[1][i];
-                ws[i][0] += v0 + v2;
-                ws[i][1] += v1 + v3;
-                uint32_t b0 = pack_f16(v0, v1), b1 = pack_f16(v2, v3);  // rows g, g + 8; this lane's columns
-                const float2 h0 = unpack_f16(b0), h1 = unpack_f16(b1);
-                uint32_t c0 = 0, c1 = 0;
-                if constexpr (kWide) {
-                    c0 = movmatrix(pack_f16(v0 - h0.x, v1 - h0.y));
-                    c1 = movmatrix(pack_f16(v2 - h1.x, v3 - h1.y));
-                } else {  // lanes of the lo columns hand over what the hi columns' rounding left
-                    b0 = pack_f16(fmaf(h0.x, lo_lane, v0), fmaf(h0.y, lo_lane, v1));
-                    b1 = pack_f16(fmaf(h1.x, lo_lane, v2), fmaf(h1.y, lo_lane, v3));
+                    for (int gr = 0; gr < 2; ++gr) {
+                        const int i = ch * 2 + gr;
+                        uint32_t h0, h1, l0, l1;
+                        split(i, p, vs, h0, h1, l0, l1);
+                        h0 = movmatrix(h0), h1 = movmatrix(h1), l0 = movmatrix(l0), l1 = movmatrix(l1);
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            values(w[2 * gr + u], 2 * i + u, h0, h1);
+                            values(w[2 * gr + u], 2 * i + u, l0, l1);
+                        }
+                    }
                 }
-                b0 = movmatrix(b0);
-                b1 = movmatrix(b1);
+            }
+        } else {
+            const bool second = lane & 2;  // lanes of the lo columns take the second tile
+            float x[4], p[4], vs[2][G];
+            {
+                float xa[4], xb[4];
+                scores(tp, lane, xa);
+                scores(tp + TB, lane, xb);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const int j = 2 * i + u;
-                    const uint32_t lo = w[2 * gr + u], hi = lo >> 8;
-                    const uint32_t a0 = lo & 0x000F000Fu, a1 = lo & 0x00F000F0u, a2 = hi & 0x000F000Fu, a3 = hi & 0x00F000F0u;
-                    mma_f16(o[j], a0, a1, a2, a3, b0, b1, o[j][0], o[j][1], o[j][2], o[j][3]);
-                    if constexpr (kWide) mma_f16(o[j], a0, a1, a2, a3, c0, c1, o[j][0], o[j][1], o[j][2], o[j][3]);
+                for (int i = 0; i < 4; ++i)
+                    x[i] = (second ? xb[i] : xa[i]) + __shfl_xor_sync(0xffffffffu, second ? xa[i] : xb[i], 2);
+            }
+            weights(second ? tp + TB : tp, r, second ? k1 : k0, k1 < 0 || edge(r, k0) || edge(r, k1), !second || k1 >= 0, lane,
+                    x, p, vs);
+#pragma unroll
+            for (int ch = 0; ch < D / 64; ++ch) {
+                const uint4 wa4 = lds128(tp + Kv4<D>::kCodes + ch * 512 + lane * 16);
+                const uint4 wb4 = lds128(tp + TB + Kv4<D>::kCodes + ch * 512 + lane * 16);
+                const uint32_t wa[4] = {wa4.x, wa4.y, wa4.z, wa4.w}, wb[4] = {wb4.x, wb4.y, wb4.z, wb4.w};
+#pragma unroll
+                for (int gr = 0; gr < 2; ++gr) {
+                    const int i = ch * 2 + gr;
+                    uint32_t h0, h1, l0, l1;
+                    split(i, p, vs, h0, h1, l0, l1);
+                    // This lane's tile's other part goes two lanes over, the other tile's comes back.
+                    const uint32_t r0 = __shfl_xor_sync(0xffffffffu, second ? h0 : l0, 2);
+                    const uint32_t r1 = __shfl_xor_sync(0xffffffffu, second ? h1 : l1, 2);
+                    const uint32_t a0 = movmatrix(second ? r0 : h0), a1 = movmatrix(second ? r1 : h1);
+                    const uint32_t b0 = movmatrix(second ? l0 : r0), b1 = movmatrix(second ? l1 : r1);
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        values(wa[2 * gr + u], 2 * i + u, a0, a1);
+                        values(wb[2 * gr + u], 2 * i + u, b0, b1);
+                    }
                 }
             }
         }
+    }
+    // Weights times the value scales of group i, as hi and lo halves of rows g (0) and g + 8 (1).
+    __device__ __forceinline__ void split(int i, const float (&p)[4], const float (&vs)[2][G], uint32_t& h0, uint32_t& h1,
+                                          uint32_t& l0, uint32_t& l1) {
+        const float v0 = p[0] * vs[0][i], v1 = p[1] * vs[0][i], v2 = p[2] * vs[1][i], v3 = p[3] * vs[1][i];
+        ws[i][0] += v0 + v2;
+        ws[i][1] += v1 + v3;
+        h0 = pack_f16(v0, v1);
+        h1 = pack_f16(v2, v3);
+        const float2 f0 = unpack_f16(h0), f1 = unpack_f16(h1);
+        l0 = pack_f16(v0 - f0.x, v1 - f0.y);
+        l1 = pack_f16(v2 - f1.x, v3 - f1.y);
     }
 
     // Moves the running maxima to those of all rows and rescales the sums.
     __device__ __forceinline__ void move_max(float t0, float t1) {
 #pragma unroll
-        for (int s = 4; s < 32; s <<= 1) {
+        for (int s = kWide ? 4 : 2; s < 32; s <<= 1) {
             t0 = fmaxf(t0, __shfl_xor_sync(0xffffffffu, t0, s));
             t1 = fmaxf(t1, __shfl_xor_sync(0xffffffffu, t1, s));
         }
@@ -460,12 +522,12 @@ struct Kv4Warp {
         const int g = lane >> 2, t = lane & 3;
         const int h0 = kWide ? 2 * t : 2 * (t & 1);  // this lane's columns are heads h0, h0 + 1
         const bool mine = h0 < NREP && (kWide || t < 2);
-        l[0] = rows_sum(l[0]);
-        l[1] = rows_sum(l[1]);
+        l[0] = rows_sum<kWide>(l[0]);
+        l[1] = rows_sum<kWide>(l[1]);
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-            ws[i][0] = 8.f * rows_sum(ws[i][0]);
-            ws[i][1] = 8.f * rows_sum(ws[i][1]);
+            ws[i][0] = 8.f * rows_sum<kWide>(ws[i][0]);
+            ws[i][1] = 8.f * rows_sum<kWide>(ws[i][1]);
         }
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
@@ -493,7 +555,8 @@ struct Kv4Warp {
 template <typename In, int D, int NREP>
 __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kernel(const Kv4DecodeArgs a) {
     using Sm = Kv4DecodeSmem<D, NREP>;
-    constexpr int L = D / 8, S = Sm::kStages, TB = Kv4<D>::kTileBytes, PF = kv4_part_floats(NREP, D);
+    constexpr int L = D / 8, TB = Kv4<D>::kTileBytes, PF = kv4_part_floats(NREP, D);
+    constexpr unsigned S = Sm::kStages;
     extern __shared__ __align__(128) uint8_t smem[];
     float* qs = reinterpret_cast<float*>(smem + Sm::kQ);
     float* kn = reinterpret_cast<float*>(smem + Sm::kKn);
@@ -506,9 +569,9 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
     int* last = reinterpret_cast<int*>(smem + Sm::kMisc + 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + Sm::kBar) + warp * S;
-    uint8_t* ring = smem + Sm::kRing + size_t(warp) * S * TB;
+    uint8_t* ring = smem + Sm::kRing + size_t(warp) * S * 2 * TB;
     if (lane == 0) {
-        for (int s = 0; s < S; ++s) mbar_init(&bars[s], 1);
+        for (unsigned s = 0; s < S; ++s) mbar_init(&bars[s], 1);
         fence_mbar_init();
     }
     if (threadIdx.x == 0) *abort = 0;
@@ -518,13 +581,15 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    const long long total = kv4_total(a, lane);
-    const int G = static_cast<int>(min(static_cast<long long>(gridDim.x), max(1ll, total / kKv4MinUnits)));
+    Kv4Positions where;
+    where.load(a, lane);
+    const int total = where.total(a, lane);
+    const int share = max(kKv4MinUnits, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
     const int bx = blockIdx.x;
     // Idle rows: zeros.
     if (a.pos_rows) {
         for (int r = bx; r < a.n_rows; r += gridDim.x) {
-            const int pos = a.pos_rows[r];
+            const int pos = where.at(a, r);
             if (pos >= 0 && pos < a.n_context) continue;
             if (pos >= 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = KERR_POSITION;
             const float z[8] = {};
@@ -537,87 +602,97 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
             }
         }
     }
-    if (bx >= G) return;
-    const long long u0 = total * bx / G, u1 = total * (bx + 1) / G;
-    if (u0 >= u1) return;
+    const long long from = static_cast<long long>(bx) * share;
+    if (from >= total) return;
+    const int u0 = static_cast<int>(from), u1 = static_cast<int>(min(static_cast<long long>(total), from + share));
     const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
-    const long long head_bytes = a.tiles_per_head * TB;
 
     // Two cursors walk the share's items: the copies', ahead, and the sums'.
     struct Cursor {
-        int row, head, t, t1;  // next tile of this warp in the item's share, and its end
-        long long start, units, next;  // first unit and units of the row's head; first unit of the next head
+        int row, head, t, t1;    // next pair of tiles of this warp in the item's share, and the share's end
+        int start, units, next;  // first unit and units of the row's head; first unit of the next head
         Kv4Row r;
+        const uint8_t* tiles;    // the head's first
     };
-    auto enter = [&](Cursor& c, long long u) {  // at unit u >= u0 of row c.row, whose heads start at c.start
-        c.r = kv4_row(a, kv4_pos(a, c.row));
-        c.units = c.r.nt + 1;
-        c.head = static_cast<int>((u - c.start) / c.units);
-        const long long h0 = c.start + c.head * c.units;
+    auto enter = [&](Cursor& c, int u) {  // at unit u >= u0 of row c.row, whose heads start at c.start
+        c.r = kv4_row(a, where.at(a, c.row));
+        c.units = kKv4ItemUnits + c.r.nt + 1;
+        c.head = (u - c.start) / c.units;
+        const int h0 = c.start + c.head * c.units;
         c.next = h0 + c.units;
-        c.t = static_cast<int>(u - h0) + warp;
-        c.t1 = static_cast<int>(min(static_cast<long long>(c.r.nt), u1 - h0));
+        c.t = max(0, u - h0 - kKv4ItemUnits) + 2 * warp;
+        c.t1 = min(c.r.nt, u1 - h0 - kKv4ItemUnits);
+        c.tiles = a.tiles + (static_cast<long long>(c.row) * a.kv_heads + c.head) * a.tiles_per_head * TB;
     };
     auto advance = [&](Cursor& c) {  // to the next item of the share; false at its end
-        if (c.next >= u1) return false;
+        if (c.next + kKv4ItemUnits >= u1) return false;  // nothing but an item's first units is left
         if (c.head + 1 == a.kv_heads) {
             c.start = c.next;
             do {
                 ++c.row;
-            } while (c.row + 1 < a.n_rows && kv4_units(a, kv4_pos(a, c.row)) == 0);
+            } while (c.row + 1 < a.n_rows && kv4_units(a, where.at(a, c.row)) == 0);
         }
         enter(c, c.next);
         return true;
     };
     Cursor in;
-    in.row = kv4_find_row(a, u0, in.start, lane);
+    in.row = where.find(a, u0, in.start, lane);
     enter(in, u0);
+    if (in.t1 <= 0 && in.next > u1) return;  // the share ends before the item's first tile
     Cursor at = in;
-    int issued = 0, taken = 0;
+    unsigned issued = 0, taken = 0;
     bool more = true;
-    auto fill = [&]() {  // requests tiles until the ring is full or the share's end
+    auto fill = [&]() {  // requests pairs until the ring is full or the share's end
         while (more && issued < taken + S) {
             if (in.t >= in.t1) {
                 more = advance(in);
                 continue;
             }
             if (lane == 0) {
-                const int s = issued % S;
-                const uint8_t* src = a.tiles + (static_cast<long long>(in.row) * a.kv_heads + in.head) * head_bytes +
-                                     static_cast<long long>(kv4_tile_of(in.r, in.t)) * TB;
-                mbar_arrive_expect_tx(&bars[s], TB);
-                bulk_copy_g2s(ring + s * TB, src, TB, &bars[s]);
+                const unsigned s = issued % S;
+                uint8_t* dst = ring + s * 2 * TB;
+                const bool two = in.t + 1 < in.t1;
+                mbar_arrive_expect_tx(&bars[s], two ? 2 * TB : TB);
+                bulk_copy_g2s(dst, in.tiles + static_cast<long long>(kv4_tile_of(in.r, in.t)) * TB, TB, &bars[s]);
+                if (two) bulk_copy_g2s(dst + TB, in.tiles + static_cast<long long>(kv4_tile_of(in.r, in.t + 1)) * TB, TB, &bars[s]);
             }
             ++issued;
-            in.t += kKv4Warps;
+            in.t += 2 * kKv4Warps;
         }
     };
     fill();
 
     Kv4Warp<D, NREP> acc;
-    long long seg0 = u0;  // first unit of the current item in this share
+    int seg0 = u0;  // first unit of the current item in this share
     for (int seg = 0;; ++seg) {
         const int pos = at.r.pos, g = at.head;
-        const long long item0 = at.next - at.units;
+        const int item0 = at.next - at.units + kKv4ItemUnits;  // the item's first tile
         const bool own = at.next <= u1;  // the item's last unit, the token itself, is in this share
+        const long long item = static_cast<long long>(at.row) * a.kv_heads + g;
         // Queries (and the token's own key and value) of the item.
-        for (int i = threadIdx.x; i < a.pairs; i += kKv4Threads) cs[i] = rope_turn(a.turns, i, pos, a.magnitude);
-        __syncthreads();
-        for (int job = warp; job < NREP + (own ? 2 : 0); job += kKv4Warps) {
-            const bool isq = job < NREP, isk = job == NREP;
-            const In* src = isq   ? static_cast<const In*>(a.q) + at.row * a.q_stride + (g * NREP + job) * D
-                            : isk ? static_cast<const In*>(a.k) + at.row * a.k_stride + g * D
-                                  : static_cast<const In*>(a.v) + at.row * a.v_stride + g * D;
+        for (int job = warp, round = 0; round < (NREP + 2 + kKv4Warps - 1) / kKv4Warps; job += kKv4Warps, ++round) {
+            const bool on = job < NREP + (own ? 2 : 0), isq = job < NREP, isk = job == NREP;
+            float x[8], gm[8];
+            if (on) {
+                const In* src = isq   ? static_cast<const In*>(a.q) + at.row * a.q_stride + (g * NREP + job) * D
+                                : isk ? static_cast<const In*>(a.k) + at.row * a.k_stride + g * D
+                                      : static_cast<const In*>(a.v) + at.row * a.v_stride + g * D;
+                load8(src + lane % L * 8, x);
+                if (a.norm) load8((isq ? a.q_gamma : a.k_gamma) + lane % L * 8, gm);
+            }
+            if (round == 0) {  // with the loads in flight
+                for (int i = threadIdx.x; i < a.pairs; i += kKv4Threads) cs[i] = rope_turn(a.turns, i, pos, a.magnitude);
+                __syncthreads();
+            }
+            if (!on) continue;
             float* dst = isq ? qs + job * D : isk ? kn : vn;
             const bool rot = isq || isk;
-            float x[8];
-            kv4_head<In, D>(src, isq ? a.q_gamma : a.k_gamma, rot && a.norm, a.eps, cs, rot ? a.pairs : 0, a.layout, dst, x, lane);
+            kv4_head<D>(x, gm, rot && a.norm, a.eps, cs, rot ? a.pairs : 0, a.layout, dst, lane);
             if (!isq) {
                 uint32_t codes;
                 const __half d = kv4_quantize8(x, codes);
                 if (lane < L) {
-                    uint8_t* tile = a.tiles + (static_cast<long long>(at.row) * a.kv_heads + g) * head_bytes +
-                                    static_cast<long long>(pos / kKv4Tile) * TB;
+                    uint8_t* tile = const_cast<uint8_t*>(at.tiles) + static_cast<long long>(pos / kKv4Tile) * TB;
                     if (isk)
                         kv4_store8<D, false>(tile, pos % kKv4Tile, lane, codes, d);
                     else
@@ -626,7 +701,7 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
                     if (rows) {
                         float y[8];
                         kv4_values8(codes, d, y);
-                        store_rows8(rows, a.rows_type, (static_cast<long long>(at.row) * a.kv_heads + g) * D + lane * 8, y);
+                        store_rows8(rows, a.rows_type, item * D + lane * 8, y);
                     }
                 }
             } else {
@@ -637,19 +712,17 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
         }
         __syncthreads();
         acc.start(qs, lane);
-        bool ok = true;
-        for (; at.t < at.t1; at.t += kKv4Warps) {
-            const int s = taken % S;
-            ok = mbar_wait_bounded(&bars[s], (taken / S) & 1, deadline, abort);
-            if (!__all_sync(0xffffffffu, ok)) {
+        for (; at.t < at.t1; at.t += 2 * kKv4Warps) {
+            const unsigned s = taken % S;
+            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bars[s], (taken / S) & 1, deadline, abort))) {
                 if (lane == 0) {
                     *abort = 1;
                     *reinterpret_cast<volatile int*>(a.err) = KERR_TIMEOUT_FULL;
                 }
-                ok = false;
                 break;
             }
-            acc.tile(ring + s * TB, at.r, kv4_tile_of(at.r, at.t) * kKv4Tile, lane);
+            acc.pair(ring + s * 2 * TB, at.r, kv4_tile_of(at.r, at.t) * kKv4Tile,
+                     at.t + 1 < at.t1 ? kv4_tile_of(at.r, at.t + 1) * kKv4Tile : -1, lane);
             __syncwarp();
             ++taken;
             fill();
@@ -666,16 +739,16 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
         __syncthreads();
         if (*abort) break;  // raised before the barrier: every thread sees it
         // Join the warps.
-        const int parts = own ? kKv4Warps + 1 : kKv4Warps;
-        const bool whole = own && seg0 == item0;  // no other block has a part of this item
-        const long long item = static_cast<long long>(at.row) * a.kv_heads + g;
+        const bool whole = own && seg0 <= item0;  // no other block has a part of this item
         In* out = static_cast<In*>(a.out) + item * NREP * D;
         float* mine = a.parts + (static_cast<long long>(bx) * 2 + (seg ? 1 : 0)) * PF;
         for (int i = threadIdx.x; i < NREP * D; i += kKv4Threads) {
             const int h = i / D;
+            const int parts = own ? kKv4Warps + 1 : kKv4Warps;
             float M = sm[h];
             for (int w = 1; w < parts; ++w) M = fmaxf(M, sm[w * NREP + h]);
             float lsum = 0.f, osum = 0.f;
+#pragma unroll
             for (int w = 0; w < kKv4Warps; ++w) {
                 const float f = ex2(sm[w * NREP + h] - M);
                 lsum = fmaf(sl[w * NREP + h], f, lsum);
@@ -694,37 +767,32 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
             }
         }
         if (!whole) {
-            __threadfence();
-            __syncthreads();
             // Blocks b0..b1 have parts of the item: those whose shares meet [item0, at.next).
-            const int b0 = static_cast<int>((item0 * G + G - 1) / total), b1 = static_cast<int>(((at.next - 1) * G + G - 1) / total);
-            // (the share of block b is [total * b / G, total * (b + 1) / G), rounded down)
-            int f = b0, e = b1;
-            while (f > 0 && total * f / G > item0) --f;
-            while (f + 1 < G && total * (f + 1) / G <= item0) ++f;
-            while (e > 0 && total * e / G > at.next - 1) --e;
-            while (e + 1 < G && total * (e + 1) / G <= at.next - 1) ++e;
+            const int b0 = item0 / share, b1 = (at.next - 1) / share, n = b1 - b0 + 1;
+            __syncthreads();
             if (threadIdx.x == 0) {
-                const int n = atomicAdd(a.tickets + item, 1);
-                *last = n == e - f;
+                __threadfence();  // the block's part (the barrier orders it before this) is out before the ticket
+                *last = atomicAdd(a.tickets + item, 1) == n - 1;
                 if (*last) a.tickets[item] = 0;
+                __threadfence();
             }
             __syncthreads();
             if (*last) {
-                __threadfence();
-                const int n = e - f + 1;
-                // Block f's part lies in its second slot when the item began inside its share.
-                const float* p0 = a.parts + (static_cast<long long>(f) * 2 + (total * f / G < item0 ? 1 : 0)) * PF;
-                auto part = [&](int i) { return i ? a.parts + static_cast<long long>(f + i) * 2 * PF : p0; };
+                // Block b0's part lies in its second slot when the item is not the first of its share.
+                const int lead = b0 * share < at.next - at.units ? 1 : 0;
                 for (int i = threadIdx.x; i < NREP * D; i += kKv4Threads) {
                     const int h = i / D;
-                    float M = -INFINITY, lsum = 0.f, osum = 0.f;
-                    for (int w = 0; w < n; ++w) M = fmaxf(M, __ldcg(part(w) + NREP * D + h));
+                    const float* p = a.parts + static_cast<long long>(b0) * 2 * PF;
+                    float M = __ldcg(p + lead * PF + NREP * D + h);
+#pragma unroll 8
+                    for (int w = 1; w < n; ++w) M = fmaxf(M, __ldcg(p + w * 2 * PF + NREP * D + h));
+                    float lsum = 0.f, osum = 0.f;
+#pragma unroll 8
                     for (int w = 0; w < n; ++w) {
-                        const float* p = part(w);
-                        const float fw = ex2(__ldcg(p + NREP * D + h) - M);
-                        lsum = fmaf(__ldcg(p + NREP * D + NREP + h), fw, lsum);
-                        osum = fmaf(__ldcg(p + i), fw, osum);
+                        const float* q = p + (w ? w * 2 : lead) * PF;
+                        const float f = ex2(__ldcg(q + NREP * D + h) - M);
+                        lsum = fmaf(__ldcg(q + NREP * D + NREP + h), f, lsum);
+                        osum = fmaf(__ldcg(q + i), f, osum);
                     }
                     out[i] = KvTraits<In>::from_float(osum / lsum);
                 }

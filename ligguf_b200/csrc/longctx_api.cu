@@ -200,7 +200,7 @@ int launch_kv4_decode(const ligguf_kv4* h, const lg::Kv4DecodeArgs& a, cudaStrea
     }
     // As many blocks as fit at once, fewer when the longest visible contexts do not fill them.
     const long long keys = std::min<long long>(h->cfg.n_context, a.window ? 2ll * lg::kKv4Tile + a.window + a.sinks : INT32_MAX);
-    const long long units = (keys / lg::kKv4Tile + 2) * a.kv_heads * a.n_rows;
+    const long long units = (keys / lg::kKv4Tile + 2 + lg::kKv4ItemUnits) * a.kv_heads * a.n_rows;
     const int slots = h->num_sms * kv4_blocks_per_sm(NREP);
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3(static_cast<unsigned>(std::min<long long>(slots, std::max<long long>(1, units / lg::kKv4MinUnits))));
@@ -415,6 +415,8 @@ int ligguf_cuda_kv4_init(const ligguf_kv4_cfg* cfg, ligguf_kv4** out) {
         ligguf_cuda_kv4_free(h);
         return code;
     };
+    if ((h->tiles_per_head + 2 + lg::kKv4ItemUnits) * c.n_kv_heads * static_cast<long long>(c.n_seqs) > INT32_MAX)
+        return bail(fail(LIGGUF_ATTN_EUNSUPPORTED, "%d sequences x %d heads x %d positions in one cache", c.n_seqs, c.n_kv_heads, c.n_context));
     // The product in double first: a cache beyond any memory must not wrap around.
     const double want = double(c.n_layers) * c.n_seqs * c.n_kv_heads * double(h->tiles_per_head) * double(h->tile_bytes);
     if (want > 1e15) return bail(fail(LIGGUF_ATTN_ENOMEM, "4-bit cache of %.3g bytes does not fit", want));
