@@ -53,6 +53,7 @@ struct Kv4DecodeArgs {
     long long tiles_per_head;
     float* parts;    // [blocks][2] partial results
     int* tickets;    // [n_rows * kv_heads], zero between calls
+    float per_block; // 1 / blocks of the launch
     int* err;
 };
 
@@ -66,23 +67,32 @@ constexpr int kKv4MinUnits = 2 * kKv4Warps;  // units a block has at least: fewe
 // item, in tiles.
 constexpr int kKv4ItemUnits = 24;
 
-// Floats of one partial result: o [NREP][D], m [NREP], l [NREP].
-__host__ __device__ constexpr int kv4_part_floats(int nrep, int dim) { return nrep * (dim + 2); }
+// Floats of one partial result: o [NREP][D], m [NREP], l [NREP], in whole 16 bytes.
+__host__ __device__ constexpr int kv4_part_floats(int nrep, int dim) { return (nrep * (dim + 2) + 3) / 4 * 4; }
 
 template <int D, int NREP>
 struct Kv4DecodeSmem {
     static constexpr int kStages = D == 128 ? 2 : 4;  // pairs of tiles a warp has in flight
+    static constexpr int kParts = NREP > 4 ? 2 : 1;   // hi and lo queries as columns of one operand, or two operands
+    static constexpr int kRow = D + 8;                // floats of a head's row of kO: two heads apart, other banks
     static constexpr size_t kRing = 0;
-    static constexpr size_t kQ = kRing + size_t(kKv4Warps) * kStages * 2 * Kv4<D>::kTileBytes;
-    static constexpr size_t kKn = kQ + NREP * D * 4;
+    static constexpr size_t kFrag = kRing + size_t(kKv4Warps) * kStages * 2 * Kv4<D>::kTileBytes;  // [kParts][D/16][32] uint2
+    static constexpr size_t kSum = kFrag + size_t(kParts) * (D / 16) * 32 * 8;                     // [8][D/32]
+    static constexpr size_t kScale = kSum + 8 * (D / 32) * 4;                                      // [8]
+    static constexpr size_t kQ = kScale + 8 * 4;
+    static constexpr size_t kGamma = kQ + NREP * D * 4;  // norm weights of q and k
+    static constexpr size_t kKn = kGamma + 2 * D * 4;
     static constexpr size_t kVn = kKn + D * 4;
     static constexpr size_t kCs = kVn + D * 4;
-    static constexpr size_t kO = kCs + D / 2 * 8;                           // [warps][NREP][D]
-    static constexpr size_t kM = kO + size_t(kKv4Warps) * NREP * D * 4;     // [warps + 1][NREP]
+    static constexpr size_t kO = kCs + D / 2 * 8;                             // [warps][NREP][kRow]
+    static constexpr size_t kW = kO + size_t(kKv4Warps) * NREP * kRow * 4;    // [warps][NREP][D/32]
+    static constexpr size_t kM = kW + size_t(kKv4Warps) * NREP * (D / 32) * 4;  // [warps + 1][NREP]
     static constexpr size_t kL = kM + (kKv4Warps + 1) * NREP * 4;
-    static constexpr size_t kBar = (kL + (kKv4Warps + 1) * NREP * 4 + 7) / 8 * 8;
+    static constexpr size_t kJoin = (kL + (kKv4Warps + 1) * NREP * 4 + 15) / 16 * 16;  // sums of a join's groups
+    static constexpr size_t kBar = kJoin + kKv4Threads * 16;
     static constexpr size_t kMisc = kBar + kKv4Warps * kStages * 8;
-    static constexpr size_t kTotal = kMisc + 16;
+    static constexpr size_t kFactors = kMisc + 16;  // [NREP] 1 / sum, then [blocks][NREP]
+    static constexpr size_t total(int blocks) { return kFactors + size_t(blocks + 1) * NREP * 4; }
 };
 
 // Visible cached tiles of a row at position p: tiles [0, ns) hold the sinks, [tw, tw + nt - ns) the window.
@@ -160,9 +170,9 @@ struct Kv4Positions {
 };
 
 // One head, 8 elements a lane (D/8 lanes, the other lanes the same again): norm and rotation of x; `dst`
-// (shared, D floats) carries the exchange.
+// (shared, D floats) carries the exchange; the norm weights are in shared memory too.
 template <int D>
-__device__ __forceinline__ void kv4_head(float (&x)[8], const float (&gamma)[8], bool norm, float eps, const float2* cs,
+__device__ __forceinline__ void kv4_head(float (&x)[8], const float* gamma, bool norm, float eps, const float2* cs,
                                          int pairs, int layout, float* dst, int lane) {
     constexpr int L = D / 8;
     const int l = lane % L;
@@ -172,8 +182,10 @@ __device__ __forceinline__ void kv4_head(float (&x)[8], const float (&gamma)[8],
         for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
         ss = head_sum<L>(ss);
         const float rs = 1.0f / sqrtf(ss / static_cast<float>(D) + eps);
+        float gm[8];
+        load8(gamma + l * 8, gm);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (x[i] * rs) * gamma[i];
+        for (int i = 0; i < 8; ++i) x[i] = (x[i] * rs) * gm[i];
     }
     if (layout == LIGGUF_ROPE_ADJACENT) {
 #pragma unroll
@@ -198,6 +210,21 @@ __device__ __forceinline__ void kv4_head(float (&x)[8], const float (&gamma)[8],
             }
         }
         __syncwarp();
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, float4 x) {
+    if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<float4*>(p) = x;
+    } else {
+        union {
+            T h[4];
+            uint2 v;
+        } u;
+        u.h[0] = KvTraits<T>::from_float(x.x), u.h[1] = KvTraits<T>::from_float(x.y);
+        u.h[2] = KvTraits<T>::from_float(x.z), u.h[3] = KvTraits<T>::from_float(x.w);
+        *reinterpret_cast<uint2*>(p) = u.v;
     }
 }
 
@@ -240,12 +267,84 @@ __device__ __forceinline__ uint2 lds64(const void* p) {
     return r;
 }
 
-// Sum over the lanes whose heads are the same: the 8 row groups, and (kWide: not) the pair's two tiles.
-template <bool kWide>
-__device__ __forceinline__ float rows_sum(float v) {
+// One query head (8 elements a lane, D/8 lanes, the others the same again), times scale * log2(e), as B
+// operands: column `head` of the hi parts and of the lo parts (column 4 + head, or a second operand).
+// Column k = 2t + b + 8c of k-step j is element 16j + 4t + 2b + c, and meets codes * 2^-24 (c = 0) or
+// * 2^-20 (c = 1).  sums: -8 * 2^-24 * the sum of a group's elements; scales: what the scores are short of.
+template <int D, int NREP>
+__device__ __forceinline__ void kv4_query_operands(const float (&x)[8], int head, uint2* frag, float* sums, float* scales,
+                                                   int lane) {
+    constexpr bool kWide = NREP > 4;
+    constexpr int L = D / 8, G = D / 32;
+    const int l = lane % L;
+    float top = 0.f;
 #pragma unroll
-    for (int o = kWide ? 4 : 2; o < 32; o <<= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[i]));
+#pragma unroll
+    for (int o = 1; o < L; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // A power of two that brings the head's largest element to [2^10, 2^11): hi is then a normal half and lo
+    // loses nothing either.
+    const int e = min(100, max(-100, ((__float_as_int(top) >> 23) & 255) - 127));
+    const float up = __int_as_float((127 + 10 - e) << 23);
+    float sh = 0.f, sl = 0.f;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const float d0 = x[4 * u] * up, d1 = x[4 * u + 1] * up * 0.0625f, d2 = x[4 * u + 2] * up, d3 = x[4 * u + 3] * up * 0.0625f;
+        const uint2 hi = make_uint2(pack_f16(d0, d2), pack_f16(d1, d3));
+        const float2 h0 = unpack_f16(hi.x), h1 = unpack_f16(hi.y);
+        const uint2 lo = make_uint2(pack_f16(d0 - h0.x, d2 - h0.y), pack_f16(d1 - h1.x, d3 - h1.y));
+        const float2 r0 = unpack_f16(lo.x), r1 = unpack_f16(lo.y);
+        sh += (h0.x + h0.y) + 16.f * (h1.x + h1.y);
+        sl += (r0.x + r0.y) + 16.f * (r1.x + r1.y);
+        const int at = (l >> 1) * 32 + 2 * (l & 1) + u;
+        if (lane < L) {
+            frag[at + head * 4] = hi;
+            frag[at + (kWide ? D / 16 * 32 + head * 4 : (4 + head) * 4)] = lo;
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+        sh += __shfl_xor_sync(0xffffffffu, sh, o);
+        sl += __shfl_xor_sync(0xffffffffu, sl, o);
+    }
+    constexpr float k8 = -8.f / 16777216.f;
+    if (lane < L && (l & 3) == 0) {
+        if (kWide) {
+            sums[head * G + (l >> 2)] = k8 * (sh + sl);
+        } else {
+            sums[head * G + (l >> 2)] = k8 * sh;
+            sums[(4 + head) * G + (l >> 2)] = k8 * sl;
+        }
+    }
+    if (lane == 0) {
+        const float down = __int_as_float((127 + e + 14) << 23);  // 2^(e - 10) * 2^24
+        scales[head] = down;
+        if (!kWide) scales[4 + head] = down;
+    }
+}
+
+// Sums of V values over the lanes that differ in bits 4..16 (the row groups) and, with kPairs, 2: each lane
+// is left with the sum of one value, number value_of(lane).
+template <int V, bool kPairs>
+__device__ __forceinline__ float rows_sum(float (&v)[V], int lane) {
+    static_assert(V == 2 || V == 4 || V == 8, "");
+    int bit = 16;
+#pragma unroll
+    for (int n = V / 2; n >= 1; n /= 2, bit /= 2) {
+        const bool up = lane & bit;
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float send = up ? v[i] : v[n + i], keep = up ? v[n + i] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, send, bit);
+        }
+    }
+#pragma unroll
+    for (; bit >= (kPairs ? 2 : 4); bit /= 2) v[0] += __shfl_xor_sync(0xffffffffu, v[0], bit);
+    return v[0];
+}
+template <int V>
+__device__ __forceinline__ int rows_value(int lane) {
+    return (lane >> 2) / (8 / V);
 }
 
 // One warp's running sums over the tiles it takes of an item.
@@ -259,62 +358,22 @@ struct Kv4Warp {
     float m[2], l[2], ws[G][2];        // running maxima, sums of weights and of weights * value scales
     float o[KS][4];
 
-    // q: [NREP][D] in shared memory, times scale * log2(e).
-    __device__ __forceinline__ void start(const float* q, int lane) {
-        const int g = lane >> 2, t = lane & 3;
-        const int head = kWide ? g : g & 3;
-        const bool is_lo = !kWide && g >= 4;
-        float top = 0.f;
-        float4 x[KS];
+    // From what kv4_query_operands left in shared memory.
+    __device__ __forceinline__ void start(const uint2* frag, const float* sums, const float* scales, int lane) {
+        const int t = lane & 3;
 #pragma unroll
-        for (int j = 0; j < KS; ++j) {
-            x[j] = head < NREP ? *reinterpret_cast<const float4*>(q + head * D + 16 * j + 4 * t) : make_float4(0.f, 0.f, 0.f, 0.f);
-            top = fmaxf(top, fmaxf(fmaxf(fabsf(x[j].x), fabsf(x[j].y)), fmaxf(fabsf(x[j].z), fabsf(x[j].w))));
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // A power of two that brings the head's largest element to [2^10, 2^11): hi is then a normal half
-        // and lo loses nothing either.
-        const int e = min(100, max(-100, ((__float_as_int(top) >> 23) & 255) - 127));
-        const float up = __int_as_float((127 + 10 - e) << 23);
-        float sum[2][G] = {};
+        for (int p = 0; p < (kWide ? 2 : 1); ++p)
 #pragma unroll
-        for (int j = 0; j < KS; ++j) {
-            const float v[4] = {x[j].x * up, x[j].y * up, x[j].z * up, x[j].w * up};
-            uint32_t part[2][2];
-#pragma unroll
-            for (int p = 0; p < 2; ++p) {  // columns 2t + b: elements 4t + 2b (codes * 2^-24), 4t + 2b + 1 (* 2^-20)
-                const float f = p ? 0.0625f : 1.f;
-                const uint32_t hi = pack_f16(v[p] * f, v[2 + p] * f);
-                const float2 h = unpack_f16(hi);
-                const uint32_t lo = pack_f16(v[p] * f - h.x, v[2 + p] * f - h.y);
-                const float2 r = unpack_f16(lo);
-                part[0][p] = hi;
-                part[1][p] = lo;
-                sum[0][j / 2] += (h.x + h.y) * (p ? 16.f : 1.f);
-                sum[1][j / 2] += (r.x + r.y) * (p ? 16.f : 1.f);
+            for (int j = 0; j < KS; ++j) {
+                const uint2 f = frag[(p * KS + j) * 32 + lane];
+                b[p][j][0] = f.x, b[p][j][1] = f.y;
             }
-            if constexpr (kWide) {
-                b[0][j][0] = part[0][0], b[0][j][1] = part[0][1];
-                b[1][j][0] = part[1][0], b[1][j][1] = part[1][1];
-            } else {
-                b[0][j][0] = is_lo ? part[1][0] : part[0][0];
-                b[0][j][1] = is_lo ? part[1][1] : part[0][1];
-            }
-        }
-        // The sums of a column lie in the four lanes of its row group; this lane's columns are 2t, 2t+1.
 #pragma unroll
         for (int i = 0; i < G; ++i) {
-            float v = kWide ? sum[0][i] + sum[1][i] : (is_lo ? sum[1][i] : sum[0][i]);
-            v += __shfl_xor_sync(0xffffffffu, v, 1);
-            v += __shfl_xor_sync(0xffffffffu, v, 2);
-            v *= -8.f / 16777216.f;
-            c[i][0] = __shfl_sync(0xffffffffu, v, 8 * t);
-            c[i][1] = __shfl_sync(0xffffffffu, v, 8 * t + 4);
+            c[i][0] = sums[2 * t * G + i];
+            c[i][1] = sums[(2 * t + 1) * G + i];
         }
-        const float down = __int_as_float((127 + e + 14) << 23);  // 2^(e - 10) * 2^24
-        sx[0] = __shfl_sync(0xffffffffu, down, 8 * t);
-        sx[1] = __shfl_sync(0xffffffffu, down, 8 * t + 4);
+        sx[0] = scales[2 * t], sx[1] = scales[2 * t + 1];
 #pragma unroll
         for (int i = 0; i < 2; ++i) m[i] = -1e30f, l[i] = 0.f;
 #pragma unroll
@@ -517,37 +576,34 @@ struct Kv4Warp {
         return make_float2(e[0], e[1]);
     }
 
-    // Sums over the warp's rows, to shared memory: o [NREP][D], m and l [NREP] (sums relative to 2^m).
-    __device__ __forceinline__ void finish(float* so, float* sm, float* sl, int lane) {
+    // Sums over the warp's rows, to shared memory: o [NREP][kRow] short of -8 times sw [NREP][G], m and l
+    // [NREP]; all relative to 2^m.
+    __device__ __forceinline__ void finish(float* so, float* sw, float* sm, float* sl, int lane) {
+        constexpr int kRow = Kv4DecodeSmem<D, NREP>::kRow;
         const int g = lane >> 2, t = lane & 3;
         const int h0 = kWide ? 2 * t : 2 * (t & 1);  // this lane's columns are heads h0, h0 + 1
-        const bool mine = h0 < NREP && (kWide || t < 2);
-        l[0] = rows_sum<kWide>(l[0]);
-        l[1] = rows_sum<kWide>(l[1]);
+        const bool first = kWide || t < 2;
+        float wv[2 * G], lv[2] = {l[0], l[1]};
 #pragma unroll
-        for (int i = 0; i < G; ++i) {
-            ws[i][0] = 8.f * rows_sum<kWide>(ws[i][0]);
-            ws[i][1] = 8.f * rows_sum<kWide>(ws[i][1]);
-        }
+        for (int i = 0; i < G; ++i) wv[2 * i] = ws[i][0], wv[2 * i + 1] = ws[i][1];
+        const float w = rows_sum<2 * G, !kWide>(wv, lane), ls = rows_sum<2, !kWide>(lv, lane);
+        const int wi = rows_value<2 * G>(lane), li = rows_value<2>(lane);
+        if (first && h0 + (wi & 1) < NREP) sw[(h0 + (wi & 1)) * G + (wi >> 1)] = 8.f * w;
+        if (first && h0 + li < NREP) sl[h0 + li] = ls, sm[h0 + li] = (li ? m[1] : m[0]) - 7.f;
+        // Rows g and g + 8 of k-step j are elements 16j + 2g, 16j + 2g + 1; their sums are short of 2^24, 2^20.
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
-            float y[4] = {o[j][0], o[j][1], o[j][2], o[j][3]};
-            if constexpr (!kWide) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) y[i] += __shfl_xor_sync(0xffffffffu, y[i], 2);
+            float* at = so + h0 * kRow + 16 * j + 2 * g;
+            if constexpr (kWide) {
+                *reinterpret_cast<float2*>(at) = make_float2(o[j][0] * 16777216.f, o[j][2] * 1048576.f);
+                *reinterpret_cast<float2*>(at + kRow) = make_float2(o[j][1] * 16777216.f, o[j][3] * 1048576.f);
+            } else {  // hi and lo columns lie two lanes apart: one lane adds rows g, the other rows g + 8
+                const float y0 = (first ? o[j][0] : o[j][2]) + __shfl_xor_sync(0xffffffffu, first ? o[j][2] : o[j][0], 2);
+                const float y1 = (first ? o[j][1] : o[j][3]) + __shfl_xor_sync(0xffffffffu, first ? o[j][3] : o[j][1], 2);
+                const float f = first ? 16777216.f : 1048576.f;
+                if (h0 < NREP) at[first ? 0 : 1] = y0 * f;
+                if (h0 + 1 < NREP) at[kRow + (first ? 0 : 1)] = y1 * f;
             }
-            if (mine) {  // rows g and g + 8 are elements 16j + 2g, 16j + 2g + 1
-                const float w0 = ws[j / 2][0], w1 = ws[j / 2][1];
-                *reinterpret_cast<float2*>(so + h0 * D + 16 * j + 2 * g) =
-                    make_float2(fmaf(y[0], 16777216.f, -w0), fmaf(y[2], 1048576.f, -w0));
-                if (h0 + 1 < NREP)
-                    *reinterpret_cast<float2*>(so + (h0 + 1) * D + 16 * j + 2 * g) =
-                        make_float2(fmaf(y[1], 16777216.f, -w1), fmaf(y[3], 1048576.f, -w1));
-            }
-        }
-        if (mine && g == 0) {
-            sm[h0] = m[0] - 7.f, sl[h0] = l[0];
-            if (h0 + 1 < NREP) sm[h0 + 1] = m[1] - 7.f, sl[h0 + 1] = l[1];
         }
     }
 };
@@ -558,6 +614,9 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
     constexpr int L = D / 8, TB = Kv4<D>::kTileBytes, PF = kv4_part_floats(NREP, D);
     constexpr unsigned S = Sm::kStages;
     extern __shared__ __align__(128) uint8_t smem[];
+    uint2* frag = reinterpret_cast<uint2*>(smem + Sm::kFrag);
+    float* sums = reinterpret_cast<float*>(smem + Sm::kSum);
+    float* scales = reinterpret_cast<float*>(smem + Sm::kScale);
     float* qs = reinterpret_cast<float*>(smem + Sm::kQ);
     float* kn = reinterpret_cast<float*>(smem + Sm::kKn);
     float* vn = reinterpret_cast<float*>(smem + Sm::kVn);
@@ -565,6 +624,7 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
     float* so = reinterpret_cast<float*>(smem + Sm::kO);
     float* sm = reinterpret_cast<float*>(smem + Sm::kM);
     float* sl = reinterpret_cast<float*>(smem + Sm::kL);
+    float* sw = reinterpret_cast<float*>(smem + Sm::kW);
     volatile int* abort = reinterpret_cast<volatile int*>(smem + Sm::kMisc);
     int* last = reinterpret_cast<int*>(smem + Sm::kMisc + 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -575,16 +635,25 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
         fence_mbar_init();
     }
     if (threadIdx.x == 0) *abort = 0;
+    if (NREP < 4) {  // columns without a head
+        for (int i = threadIdx.x; i < D / 16 * 32; i += kKv4Threads) frag[i] = make_uint2(0, 0);
+        for (int i = threadIdx.x; i < 8 * (D / 32); i += kKv4Threads) sums[i] = 0.f;
+        if (threadIdx.x < 8) scales[threadIdx.x] = 1.f;
+    }
+    // The norm weights, which no kernel writes.
+    float* gammas = reinterpret_cast<float*>(smem + Sm::kGamma);
+    if (a.norm && threadIdx.x < 2 * D) gammas[threadIdx.x] = threadIdx.x < D ? a.q_gamma[threadIdx.x] : a.k_gamma[threadIdx.x - D];
     __syncthreads();
-    // Everything before touched only this block's shared memory; the previous kernel of the stream (which
-    // may have written the cache, the positions or the rows) has completed after this.
+    // Everything before touched only this block's shared memory and what the host wrote; the previous kernel
+    // of the stream (which may have written the cache, the positions or the rows) has completed after this.
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     Kv4Positions where;
     where.load(a, lane);
     const int total = where.total(a, lane);
-    const int share = max(kKv4MinUnits, (total + static_cast<int>(gridDim.x) - 1) / static_cast<int>(gridDim.x));
+    // At least total / gridDim.x, by a product: the conversion rounds up, and one in 2^20 covers the factor's error.
+    const int share = max(kKv4MinUnits, __float2int_ru(static_cast<float>(total) * a.per_block) + (total >> 20));
     const int bx = blockIdx.x;
     // Idle rows: zeros.
     if (a.pos_rows) {
@@ -617,7 +686,9 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
     auto enter = [&](Cursor& c, int u) {  // at unit u >= u0 of row c.row, whose heads start at c.start
         c.r = kv4_row(a, where.at(a, c.row));
         c.units = kKv4ItemUnits + c.r.nt + 1;
-        c.head = (u - c.start) / c.units;
+        // The head: heads whose units end at or before u.
+        c.head = a.kv_heads <= 32 ? __popc(__ballot_sync(0xffffffffu, lane < a.kv_heads && (lane + 1) * c.units <= u - c.start))
+                                  : (u - c.start) / c.units;
         const int h0 = c.start + c.head * c.units;
         c.next = h0 + c.units;
         c.t = max(0, u - h0 - kKv4ItemUnits) + 2 * warp;
@@ -672,22 +743,21 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
         // Queries (and the token's own key and value) of the item.
         for (int job = warp, round = 0; round < (NREP + 2 + kKv4Warps - 1) / kKv4Warps; job += kKv4Warps, ++round) {
             const bool on = job < NREP + (own ? 2 : 0), isq = job < NREP, isk = job == NREP;
-            float x[8], gm[8];
+            float x[8];
             if (on) {
                 const In* src = isq   ? static_cast<const In*>(a.q) + at.row * a.q_stride + (g * NREP + job) * D
                                 : isk ? static_cast<const In*>(a.k) + at.row * a.k_stride + g * D
                                       : static_cast<const In*>(a.v) + at.row * a.v_stride + g * D;
                 load8(src + lane % L * 8, x);
-                if (a.norm) load8((isq ? a.q_gamma : a.k_gamma) + lane % L * 8, gm);
             }
             if (round == 0) {  // with the loads in flight
-                for (int i = threadIdx.x; i < a.pairs; i += kKv4Threads) cs[i] = rope_turn(a.turns, i, pos, a.magnitude);
+                if (threadIdx.x < a.pairs) cs[threadIdx.x] = rope_turn(a.turns[threadIdx.x], pos, a.magnitude);
                 __syncthreads();
             }
             if (!on) continue;
             float* dst = isq ? qs + job * D : isk ? kn : vn;
             const bool rot = isq || isk;
-            kv4_head<D>(x, gm, rot && a.norm, a.eps, cs, rot ? a.pairs : 0, a.layout, dst, lane);
+            kv4_head<D>(x, gammas + (isq ? 0 : D), rot && a.norm, a.eps, cs, rot ? a.pairs : 0, a.layout, dst, lane);
             if (!isq) {
                 uint32_t codes;
                 const __half d = kv4_quantize8(x, codes);
@@ -707,11 +777,12 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[i] *= a.scale_log2;
+                kv4_query_operands<D, NREP>(x, job, frag, sums, scales, lane);
             }
             if (lane < L) store8(dst + lane * 8, x);
         }
         __syncthreads();
-        acc.start(qs, lane);
+        acc.start(frag, sums, scales, lane);
         for (; at.t < at.t1; at.t += 2 * kKv4Warps) {
             const unsigned s = taken % S;
             if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bars[s], (taken / S) & 1, deadline, abort))) {
@@ -727,7 +798,7 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
             ++taken;
             fill();
         }
-        acc.finish(so + warp * NREP * D, sm + warp * NREP, sl + warp * NREP, lane);
+        acc.finish(so + warp * NREP * Sm::kRow, sw + warp * NREP * (D / 32), sm + warp * NREP, sl + warp * NREP, lane);
         if (own)  // the token itself: one key whose weight is 1 relative to its own score
             for (int h = warp; h < NREP; h += kKv4Warps) {
                 float x = 0.f;
@@ -743,27 +814,23 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
         In* out = static_cast<In*>(a.out) + item * NREP * D;
         float* mine = a.parts + (static_cast<long long>(bx) * 2 + (seg ? 1 : 0)) * PF;
         for (int i = threadIdx.x; i < NREP * D; i += kKv4Threads) {
-            const int h = i / D;
-            const int parts = own ? kKv4Warps + 1 : kKv4Warps;
-            float M = sm[h];
-            for (int w = 1; w < parts; ++w) M = fmaxf(M, sm[w * NREP + h]);
-            float lsum = 0.f, osum = 0.f;
+            const int h = i / D, d = i % D;
+            float M = own ? sm[kKv4Warps * NREP + h] : -1e30f, mw[kKv4Warps];
+#pragma unroll
+            for (int w = 0; w < kKv4Warps; ++w) mw[w] = sm[w * NREP + h], M = fmaxf(M, mw[w]);
+            const float f0 = own ? ex2(sm[kKv4Warps * NREP + h] - M) : 0.f;
+            float lsum = f0, osum = own ? f0 * vn[d] : 0.f;
 #pragma unroll
             for (int w = 0; w < kKv4Warps; ++w) {
-                const float f = ex2(sm[w * NREP + h] - M);
+                const float f = ex2(mw[w] - M);
                 lsum = fmaf(sl[w * NREP + h], f, lsum);
-                osum = fmaf(so[w * NREP * D + i], f, osum);
-            }
-            if (own) {
-                const float f = ex2(sm[kKv4Warps * NREP + h] - M);
-                lsum += f;
-                osum = fmaf(vn[i % D], f, osum);
+                osum = fmaf(so[(w * NREP + h) * Sm::kRow + d] - sw[(w * NREP + h) * (D / 32) + d / 32], f, osum);
             }
             if (whole) {
                 out[i] = KvTraits<In>::from_float(osum / lsum);
             } else {
                 mine[i] = osum;
-                if (i % D == 0) mine[NREP * D + h] = M, mine[NREP * D + NREP + h] = lsum;
+                if (d == 0) mine[NREP * D + h] = M, mine[NREP * D + NREP + h] = lsum;
             }
         }
         if (!whole) {
@@ -771,30 +838,64 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
             const int b0 = item0 / share, b1 = (at.next - 1) / share, n = b1 - b0 + 1;
             __syncthreads();
             if (threadIdx.x == 0) {
-                __threadfence();  // the block's part (the barrier orders it before this) is out before the ticket
-                *last = atomicAdd(a.tickets + item, 1) == n - 1;
-                if (*last) a.tickets[item] = 0;
-                __threadfence();
+                // The block's part, ordered before this by the barrier, is out before the ticket; what the
+                // other blocks put out before theirs is seen after it.
+                int done;
+                asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(done) : "l"(a.tickets + item) : "memory");
+                *last = done == n - 1;
+                if (done == n - 1) a.tickets[item] = 0;
             }
             __syncthreads();
             if (*last) {
                 // Block b0's part lies in its second slot when the item is not the first of its share.
                 const int lead = b0 * share < at.next - at.units ? 1 : 0;
-                for (int i = threadIdx.x; i < NREP * D; i += kKv4Threads) {
-                    const int h = i / D;
-                    const float* p = a.parts + static_cast<long long>(b0) * 2 * PF;
-                    float M = __ldcg(p + lead * PF + NREP * D + h);
-#pragma unroll 8
-                    for (int w = 1; w < n; ++w) M = fmaxf(M, __ldcg(p + w * 2 * PF + NREP * D + h));
-                    float lsum = 0.f, osum = 0.f;
-#pragma unroll 8
-                    for (int w = 0; w < n; ++w) {
-                        const float* q = p + (w ? w * 2 : lead) * PF;
-                        const float f = ex2(__ldcg(q + NREP * D + h) - M);
-                        lsum = fmaf(__ldcg(q + NREP * D + NREP + h), f, lsum);
-                        osum = fmaf(__ldcg(q + i), f, osum);
+                const float* parts = a.parts + static_cast<long long>(b0) * 2 * PF;
+                auto part = [&](int w) { return parts + (w ? w * 2 : lead) * PF; };
+                // Threads in groups, one 16-byte column a thread; a group takes every kGroups-th part.
+                constexpr int kCols = NREP * D / 4, kGroups = kKv4Threads / kCols, kAhead = 8;
+                const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+                float4 x[kAhead];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u)
+                    if (grp + u * kGroups < n) x[u] = __ldcg(reinterpret_cast<const float4*>(part(grp + u * kGroups)) + col);
+                float* inv = reinterpret_cast<float*>(smem + Sm::kFactors);
+                float* fac = inv + NREP;
+                if (warp < NREP) {  // the parts' factors, a head a warp
+                    float M = -1e30f, ls = 0.f;
+                    for (int w = lane; w < n; w += 32) M = fmaxf(M, __ldcg(part(w) + NREP * D + warp));
+                    M = warp_max(M);
+                    for (int w = lane; w < n; w += 32) {
+                        const float f = ex2(__ldcg(part(w) + NREP * D + warp) - M);
+                        fac[w * NREP + warp] = f;
+                        ls = fmaf(__ldcg(part(w) + NREP * D + NREP + warp), f, ls);
                     }
-                    out[i] = KvTraits<In>::from_float(osum / lsum);
+                    ls = warp_sum(ls);
+                    if (lane == 0) inv[warp] = 1.f / ls;
+                }
+                __syncthreads();
+                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                const int h = col * 4 / D;
+                for (int w0 = grp; w0 < n; w0 += kGroups * kAhead) {
+#pragma unroll
+                    for (int u = 0; u < kAhead; ++u) {
+                        const int w = w0 + u * kGroups;
+                        if (w >= n) continue;
+                        const float f = fac[w * NREP + h];
+                        const float4 z = w0 == grp ? x[u] : __ldcg(reinterpret_cast<const float4*>(part(w)) + col);
+                        y.x = fmaf(z.x, f, y.x), y.y = fmaf(z.y, f, y.y), y.z = fmaf(z.z, f, y.z), y.w = fmaf(z.w, f, y.w);
+                    }
+                }
+                float4* join = reinterpret_cast<float4*>(smem + Sm::kJoin);
+                join[threadIdx.x] = y;
+                __syncthreads();
+                if (grp == 0) {
+#pragma unroll
+                    for (int i = 1; i < kGroups; ++i) {
+                        const float4 z = join[i * kCols + col];
+                        y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+                    }
+                    const float f = inv[h];
+                    store4(out + col * 4, make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
                 }
             }
         }

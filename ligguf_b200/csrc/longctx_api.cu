@@ -189,13 +189,13 @@ int kv4_check(const ligguf_kv4* h, int layer, int seq, int n_seqs, int pos0, int
 }
 
 template <typename In, int D, int NREP>
-int launch_kv4_decode(const ligguf_kv4* h, const lg::Kv4DecodeArgs& a, cudaStream_t st) {
+int launch_kv4_decode(const ligguf_kv4* h, lg::Kv4DecodeArgs& a, cudaStream_t st) {
     using Sm = lg::Kv4DecodeSmem<D, NREP>;
     auto kern = lg::kv4_decode_kernel<In, D, NREP>;
     static bool attr_done[64] = {};
     const int device = h->cfg.device;
     if (device >= 64 || !attr_done[device]) {
-        LG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Sm::kTotal)));
+        LG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Sm::total(h->num_sms * kv4_blocks_per_sm(NREP)))));
         if (device < 64) attr_done[device] = true;
     }
     // As many blocks as fit at once, fewer when the longest visible contexts do not fill them.
@@ -204,8 +204,9 @@ int launch_kv4_decode(const ligguf_kv4* h, const lg::Kv4DecodeArgs& a, cudaStrea
     const int slots = h->num_sms * kv4_blocks_per_sm(NREP);
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3(static_cast<unsigned>(std::min<long long>(slots, std::max<long long>(1, units / lg::kKv4MinUnits))));
+    a.per_block = 1.0f / static_cast<float>(lc.gridDim.x);
     lc.blockDim = dim3(lg::kKv4Threads);
-    lc.dynamicSmemBytes = Sm::kTotal;
+    lc.dynamicSmemBytes = Sm::total(slots);
     lc.stream = st;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -216,7 +217,7 @@ int launch_kv4_decode(const ligguf_kv4* h, const lg::Kv4DecodeArgs& a, cudaStrea
     return LIGGUF_ATTN_OK;
 }
 template <typename In, int D>
-int launch_kv4_decode_n(const ligguf_kv4* h, const lg::Kv4DecodeArgs& a, cudaStream_t st) {
+int launch_kv4_decode_n(const ligguf_kv4* h, lg::Kv4DecodeArgs& a, cudaStream_t st) {
     switch (h->nrep) {
         case 1: return launch_kv4_decode<In, D, 1>(h, a, st);
         case 2: return launch_kv4_decode<In, D, 2>(h, a, st);
@@ -225,7 +226,7 @@ int launch_kv4_decode_n(const ligguf_kv4* h, const lg::Kv4DecodeArgs& a, cudaStr
     }
 }
 template <typename In>
-int launch_kv4_decode_d(const ligguf_kv4* h, const lg::Kv4DecodeArgs& a, cudaStream_t st) {
+int launch_kv4_decode_d(const ligguf_kv4* h, lg::Kv4DecodeArgs& a, cudaStream_t st) {
     return h->cfg.rope.head_dim == 64 ? launch_kv4_decode_n<In, 64>(h, a, st) : launch_kv4_decode_n<In, 128>(h, a, st);
 }
 

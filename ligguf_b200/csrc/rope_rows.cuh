@@ -34,9 +34,9 @@ struct RopeRowsArgs {
     int units_per_block;
 };
 
-// sin and cos of position * f for pair i, times the magnitude.
-__device__ __forceinline__ float2 rope_turn(const double* __restrict__ turns, int i, int pos, float magnitude) {
-    const double t = static_cast<double>(pos) * turns[i];
+// cos and sin of position * f, times the magnitude; turns = f / 2pi.
+__device__ __forceinline__ float2 rope_turn(double turns, int pos, float magnitude) {
+    const double t = static_cast<double>(pos) * turns;
     float s, c;
     sincospif(static_cast<float>(2.0 * (t - rint(t))), &s, &c);
     return make_float2(magnitude * c, magnitude * s);
@@ -61,7 +61,7 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeRowsArgs a) {
     __shared__ float xch[kLayout == kRopeHalvesOdd ? 256 * 8 : 1];
     const long long tok = blockIdx.x;
     const int pos = a.pos ? a.pos[tok] : a.pos0 + static_cast<int>(tok);
-    for (int i = threadIdx.x; i < a.pairs; i += 256) cs[i] = rope_turn(a.turns, i, pos, a.magnitude);
+    for (int i = threadIdx.x; i < a.pairs; i += 256) cs[i] = rope_turn(a.turns[i], pos, a.magnitude);
     __syncthreads();
     const int q_units = a.q ? a.q_heads * L : 0, k_units = a.kv_heads * L;
     const int total = q_units + k_units + (a.v ? k_units : 0);
