@@ -3,6 +3,7 @@
 // LIGGUF_ATTN_ECUDA, and a scoped switch of the current device.
 #pragma once
 
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 #include "ligguf_cuda_attn.h"
@@ -13,6 +14,9 @@ namespace lgapi {
 int fail(int code, const char* fmt, ...);
 // The reason recorded last on the calling thread ("" if none).
 const char* last_error();
+
+// The driver's cuTensorMapEncodeTiled, or null.
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
 struct DeviceGuard {
     int prev = -1;

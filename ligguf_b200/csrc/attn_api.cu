@@ -34,14 +34,6 @@ int fail(int code, const char* fmt, ...) {
     return code;
 }
 const char* last_error() { return g_last_error.c_str(); }
-}  // namespace lgapi
-
-namespace {
-using lgapi::DeviceGuard;
-using lgapi::fail;
-
-inline int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
-
 PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
     if (!fn) {
@@ -54,6 +46,14 @@ PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     }
     return fn;
 }
+}  // namespace lgapi
+
+namespace {
+using lgapi::DeviceGuard;
+using lgapi::fail;
+using lgapi::tensor_map_encoder;
+
+inline int ceil_div(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
 
 size_t kv_elem_size(int kv_type) { return kv_type == LIGGUF_KV_F32 ? 4 : 2; }
 

@@ -95,6 +95,15 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
         : "memory");
 }
 
+__device__ __forceinline__ void tma_load_4d(void* smem_dst, const CUtensorMap* map, uint64_t* bar,
+                                            int c0, int c1, int c2, int c3) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(smem_u32(smem_dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+        : "memory");
+}
+
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
     asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
@@ -113,6 +122,7 @@ struct KvTraits;
 
 template <>
 struct KvTraits<float> {
+    static constexpr bool kBf16 = false;
     static constexpr int kElemsPer16B = 4;
     __device__ static __forceinline__ void unpack(const uint4& r, float* x) {
         x[0] = __uint_as_float(r.x);
@@ -126,6 +136,7 @@ struct KvTraits<float> {
 
 template <>
 struct KvTraits<__half> {
+    static constexpr bool kBf16 = false;
     static constexpr int kElemsPer16B = 8;
     __device__ static __forceinline__ void unpack(const uint4& r, float* x) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};
@@ -142,6 +153,7 @@ struct KvTraits<__half> {
 
 template <>
 struct KvTraits<__nv_bfloat16> {
+    static constexpr bool kBf16 = true;
     static constexpr int kElemsPer16B = 8;
     __device__ static __forceinline__ void unpack(const uint4& r, float* x) {
         const uint32_t w[4] = {r.x, r.y, r.z, r.w};

@@ -23,6 +23,10 @@
 //               its half of O when the running max moves (rare), and keeps its half of the row sum
 //   warps 12..15 epilogue: O / l from TMEM to global memory through a padded staging block (whole
 //               128-byte row segments per store), so the softmax warps never wait for it
+// The windowed form (TcWindow; causal with a sliding window and visible first tokens, over the caller's own
+// 16-bit rows) is the same kernel: an item's key tiles are those of the first tokens and of the window, the
+// mask has a lower bound too, and warp 3 zeroes the rows of an edge tile of V that no query row of the tile
+// sees (they may hold anything, and P = 0 times NaN is NaN) before P.V reads it.
 // Items are walked heaviest first: causal prefill by their numbering, BERT through a work order
 // sorted by key-tile count that the operand conversion kernel writes (bert_item_order).
 // TMEM: S double buffer [0, 256), O double-buffered by item after it.  An issuing thread loses
@@ -49,6 +53,24 @@ struct TcArgs {
     float scale_log2;          // softmax scale times log2(e)
     int* err;
     const int* order;  // null, or order[p] = the item taken at walk position p (a permutation)
+    // windowed form only
+    const int* pos0;   // per-batch position of the first query row (null: len - q_seq)
+    int window, sinks;
+    void* wout;        // [q_rows][q_heads][D] of the form's output type
+};
+
+// What the kernel computes: TcFull, BERT and causal prefill on bf16 copies, fp32 out; TcWindow, the
+// windowed form on the caller's rows (T fp16 or bf16, out T or fp32).
+struct TcFull {
+    static constexpr bool kWindow = false;
+    using Operand = __nv_bfloat16;
+    using Out = float;
+};
+template <typename T, typename O>
+struct TcWindow {
+    static constexpr bool kWindow = true;
+    using Operand = T;
+    using Out = O;
 };
 
 constexpr int kTcRows = 128;  // query rows per tile (UMMA M)
@@ -67,7 +89,7 @@ __device__ __forceinline__ int bert_group_cost(const int* lens, int g, int n_qt,
     const int len = min(lens[b], max_len);
     return r0 >= len ? 0 : (len + kTcKeys - 1) / kTcKeys;
 }
-__device__ void bert_item_order(const int* __restrict__ lens, int batch, int max_len, int n_heads,
+static __device__ void bert_item_order(const int* __restrict__ lens, int batch, int max_len, int n_heads,
                                 int* __restrict__ order) {
     __shared__ int bins[kOrderBins];
     const int n_qt = (max_len + kTcRows - 1) / kTcRows;
@@ -104,7 +126,7 @@ __device__ void bert_item_order(const int* __restrict__ lens, int batch, int max
 // 16-byte store).  Needs E % 8 == 0 and 16-byte aligned bases.  With `order` set, the grid has one
 // more column of blocks, and its first block writes the work order (bert_item_order) instead.
 constexpr int kBertConvRows = 8;
-__global__ void __launch_bounds__(256) bert_to_bf16_kernel(const float* __restrict__ q, const float* __restrict__ k,
+static __global__ void __launch_bounds__(256) bert_to_bf16_kernel(const float* __restrict__ q, const float* __restrict__ k,
                                                            const float* __restrict__ v, const int* __restrict__ lens,
                                                            int max_len, int E, __nv_bfloat16* __restrict__ bq,
                                                            __nv_bfloat16* __restrict__ bk, __nv_bfloat16* __restrict__ bv,
@@ -197,7 +219,7 @@ struct TcSmem {
     static constexpr size_t kBar = kE + 4 * 32 * kStageRow * 4;
     // k_full[S], k_empty[S], v_full[S], v_empty[S], s_full[2], p_full[2], pv_done[2], drain, q_full[2],
     // q_empty[2], o_final[2], o_free[2], l_full[kLRing]
-    static constexpr int kNumBars = 4 * kStages + 2 + 2 + 2 + 1 + 8 + kLRing + 8;  // + xchg[2][4]
+    static constexpr int kNumBars = 4 * kStages + 2 + 2 + 2 + 1 + 8 + kLRing + 8 + 2;  // + xchg[2][4], v_ask, v_fixed
     static constexpr size_t kMisc = kBar + size_t(kNumBars) * 8;  // tmem base, abort flag
     static constexpr size_t kTotal = kMisc + 16 + 1024;           // + slack to align the base to 1 KB
 };
@@ -250,9 +272,9 @@ __device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo
 // The same descriptor `bytes` further on: the start address is the low 14-bit field (address >> 4),
 // and shared-memory addresses stay below 2^18, so the add never carries out of the field.
 __device__ __forceinline__ uint64_t desc_advance(uint64_t desc, uint32_t bytes) { return desc + (bytes >> 4); }
-// Instruction descriptor, kind::f16: bf16 A and B, fp32 accumulator, M x N, majors (0 K, 1 MN).
-__host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, int a_mn, int b_mn) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) |
+// Instruction descriptor, kind::f16: bf16 (or fp16) A and B, fp32 accumulator, M x N, majors (0 K, 1 MN).
+__host__ __device__ constexpr uint32_t idesc_16bit(bool bf16, int M, int N, int a_mn, int b_mn) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (uint32_t(a_mn) << 15) | (uint32_t(b_mn) << 16) |
            (uint32_t(N >> 3) << 17) | (uint32_t(M >> 4) << 24);
 }
 
@@ -305,6 +327,15 @@ __device__ __forceinline__ float fast_exp2(float x) {
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack_16bit(float lo, float hi) {
+    if constexpr (!KvTraits<T>::kBf16) {
+        const __half2 v = __floats2half2_rn(lo, hi);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    } else {
+        return pack_bf16(lo, hi);
+    }
 }
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
@@ -390,6 +421,12 @@ __device__ __forceinline__ float2 exp2_poly2(float2 x) {
 // the elements).  Measured: a quarter beats none, three eighths and a half.
 constexpr unsigned kTcPolyPairs = 0x88u;
 
+__device__ __forceinline__ void tc_store4(float* p, float4 x) { *reinterpret_cast<float4*>(p) = x; }
+template <typename T>
+__device__ __forceinline__ void tc_store4(T* p, float4 x) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_16bit<T>(x.x, x.y), pack_16bit<T>(x.z, x.w));
+}
+
 // One work item: 128 query rows (one tile) of one head of one batch entry.  n_kv == 0 marks an item
 // of padded query rows only, which is written as zeros and never reaches the tensor cores.
 struct TcItem {
@@ -410,6 +447,49 @@ __device__ __forceinline__ TcItem tc_item(const TcArgs& a, int idx, int n_qt) {
     it.n_kv = it.r0 >= it.nq_valid ? 0 : max(0, (kv_eff + kTcKeys - 1) / kTcKeys);
     return it;
 }
+// The windowed form's items: the same numbering; key tiles [0, ns) of the first tokens, then
+// [tw, tw + n_kv - ns).  lo, hi: keys [lo, hi) and those below `sinks` are seen by some row of the tile.
+struct TcWinItem : TcItem {
+    int p0;            // position of the tile's first row
+    int ns, tw, lo, hi;
+};
+__device__ __forceinline__ TcWinItem tc_window_item(const TcArgs& a, int idx, int n_qt) {
+    TcWinItem it;
+    it.h = idx % a.q_heads;
+    const int y = (idx / a.q_heads) % n_qt;
+    it.b = idx / (a.q_heads * n_qt);
+    it.r0 = (n_qt - 1 - y) * kTcRows;
+    it.nq_valid = a.q_seq;
+    it.kv_len = a.lens ? max(0, min(a.lens[it.b], a.kv_seq)) : a.kv_seq;
+    // A first position below -q_seq (nothing is seen) or beyond every key and window (only first tokens
+    // are) gives what the nearest bound gives; the bounds keep the sums below 2^31.
+    const int first = a.pos0 ? a.pos0[it.b] : it.kv_len - a.q_seq;
+    it.p0 = max(-a.q_seq, min(first, a.kv_seq + a.window)) + it.r0;
+    const int p1 = it.p0 + min(kTcRows, a.q_seq - it.r0) - 1;
+    it.hi = max(0, min(it.kv_len, p1 + 1));
+    it.lo = a.window ? max(0, min(it.p0 - a.window + 1, it.hi)) : 0;
+    const int te = (it.hi + kTcKeys - 1) / kTcKeys;
+    it.tw = min(it.lo / kTcKeys, te);
+    // (lo == hi on a tile boundary: no row sees a key of the window)
+    it.ns = a.window ? min((min(a.sinks, it.hi) + kTcKeys - 1) / kTcKeys, it.tw) : 0;
+    it.n_kv = it.ns + (it.lo < it.hi ? te - it.tw : 0);
+    if (it.lo >= it.hi && min(a.sinks, it.hi) > it.ns * kTcKeys) it.n_kv = it.ns + 1;  // first tokens in tile tw
+    return it;
+}
+__device__ __forceinline__ int tc_window_key0(const TcWinItem& it, int j) {
+    return (j < it.ns ? j : it.tw + (j - it.ns)) * kTcKeys;
+}
+// Whether rows of V's tile at key k0 are seen by no row of the item (and are zeroed before use).
+__device__ __forceinline__ bool tc_window_fix(const TcArgs& a, const TcWinItem& it, int k0) {
+    return k0 + kTcKeys > it.hi || (k0 < it.lo && k0 + kTcKeys > a.sinks);
+}
+template <typename Mode>
+__device__ __forceinline__ auto tc_any_item(const TcArgs& a, int idx, int n_qt) {
+    if constexpr (Mode::kWindow)
+        return tc_window_item(a, idx, n_qt);
+    else
+        return tc_item(a, idx, n_qt);
+}
 // The w-th item of this CTA.  The grid is persistent (as many CTAs as fit at once) and walks the
 // items in waves of gridDim.x, every other wave in reverse CTA order: with the heaviest items
 // first, the CTA that took the heaviest item of one wave takes the lightest of the next.
@@ -425,12 +505,13 @@ __device__ __forceinline__ int tc_walk(const TcArgs& a, int w, int n_items) {
     return a.order ? __ldg(a.order + p) : p;
 }
 
-template <int D>
+template <int D, typename Mode = TcFull>
 __global__ void __launch_bounds__(kTcThreads, 1)
     flash_tc_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                     const __grid_constant__ CUtensorMap tm_v, const TcArgs a) {
     using Sm = TcSmem<D>;
     using Tm = TcTmem<D>;
+    constexpr bool kWin = Mode::kWindow, kBf16 = KvTraits<typename Mode::Operand>::kBf16;
     constexpr int S = Sm::kStages;
     constexpr int NCH = Sm::kChunks;
     constexpr int LR = Sm::kLRing;
@@ -455,6 +536,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint64_t* o_free = o_final + 2;   // [2] the epilogue has read O
     uint64_t* l_full = o_free + 2;
     uint64_t* xchg = l_full + LR;     // [tile parity][quarter] both halves of the rows wrote their maxima    // [LR] the item's row sums are in shared memory
+    // Windowed: the P.V issuer asks for an edge tile's unseen rows of V to be zeroed, and they are.  One tile
+    // at a time, so both barriers advance a phase per edge tile.
+    uint64_t* v_ask = xchg + 8;
+    uint64_t* v_fixed = v_ask + 1;
     float* lsum = reinterpret_cast<float*>(sm + Sm::kL);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(sm + Sm::kMisc);
     volatile int* abort = reinterpret_cast<volatile int*>(sm + Sm::kMisc + 4);
@@ -488,6 +573,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         mbar_init(&pv_done[0], 1);
         mbar_init(&pv_done[1], 1);
         mbar_init(drain, 2);
+        mbar_init(v_ask, 1);
+        mbar_init(v_fixed, 1);
         *abort = 0;
         fence_mbar_init();
     }
@@ -513,7 +600,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int w = 0; ok; ++w) {
                     const int idx = tc_walk(a, w, n_items);
                     if (idx < 0) break;
-                    const TcItem it = tc_item(a, idx, n_qt);
+                    const auto it = tc_any_item<Mode>(a, idx, n_qt);
                     if (it.n_kv == 0) continue;
                     deadline = globaltimer_ns() + kWaitLimitNs;
                     // Q of item z into buffer z & 1, once the last S MMA of item z - 2 has read it.
@@ -522,9 +609,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         !tc_wait(&q_empty[qb], ((z >> 1) - 1) & 1, deadline, abort, a.err, KERR_TIMEOUT_EMPTY))
                         break;
                     mbar_arrive_expect_tx(&q_full[qb], Sm::kQBytes);
-                    for (int c = 0; c < NCH; ++c)
-                        tma_load_3d(sm + Sm::kQ + qb * Sm::kQBytes + c * Sm::kQChunkBytes, &tm_q, &q_full[qb], 64 * c,
-                                    it.h, it.b * a.q_seq + it.r0);
+                    for (int c = 0; c < NCH; ++c) {
+                        uint8_t* dst = sm + Sm::kQ + qb * Sm::kQBytes + c * Sm::kQChunkBytes;
+                        if constexpr (kWin)
+                            tma_load_4d(dst, &tm_q, &q_full[qb], 64 * c, it.h, it.r0, it.b);
+                        else
+                            tma_load_3d(dst, &tm_q, &q_full[qb], 64 * c, it.h, it.b * a.q_seq + it.r0);
+                    }
                     ++z;
                     const int g = it.h / a.nrep, kv_row0 = it.b * a.kv_seq;
                     for (int j = 0; j < it.n_kv; ++j, ++t) {
@@ -535,18 +626,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             break;
                         }
                         mbar_arrive_expect_tx(&k_full[s], Sm::kKvBytes);
-                        for (int c = 0; c < NCH; ++c)
-                            tma_load_3d(sm + Sm::kK + s * Sm::kKvBytes + c * Sm::kKvChunkBytes, &tm_k, &k_full[s],
-                                        64 * c, g, kv_row0 + j * kTcKeys);
+                        for (int c = 0; c < NCH; ++c) {
+                            uint8_t* dst = sm + Sm::kK + s * Sm::kKvBytes + c * Sm::kKvChunkBytes;
+                            if constexpr (kWin)
+                                tma_load_4d(dst, &tm_k, &k_full[s], 64 * c, g, tc_window_key0(it, j), it.b);
+                            else
+                                tma_load_3d(dst, &tm_k, &k_full[s], 64 * c, g, kv_row0 + j * kTcKeys);
+                        }
                         if (t >= S && !tc_wait(&v_empty[s], par, deadline, abort, a.err, KERR_TIMEOUT_EMPTY)) {
                             ++issued;  // the K half of this stage is in flight
                             ok = false;
                             break;
                         }
                         mbar_arrive_expect_tx(&v_full[s], Sm::kKvBytes);
-                        for (int c = 0; c < NCH; ++c)
-                            tma_load_3d(sm + Sm::kV + s * Sm::kKvBytes + c * Sm::kKvChunkBytes, &tm_v, &v_full[s],
-                                        64 * c, g, kv_row0 + j * kTcKeys);
+                        for (int c = 0; c < NCH; ++c) {
+                            uint8_t* dst = sm + Sm::kV + s * Sm::kKvBytes + c * Sm::kKvChunkBytes;
+                            if constexpr (kWin)
+                                tma_load_4d(dst, &tm_v, &v_full[s], 64 * c, g, tc_window_key0(it, j), it.b);
+                            else
+                                tma_load_3d(dst, &tm_v, &v_full[s], 64 * c, g, kv_row0 + j * kTcKeys);
+                        }
                         ++issued;
                     }
                 }
@@ -565,6 +664,38 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     }
                 }
             }
+        } else if (kWin && warp == 3) {
+            // ------------------------------------------------------------------ unseen rows of V
+            if constexpr (kWin) {
+                bool ok = true;
+                int t = 0, asked = 0;
+                for (int w = 0; ok; ++w) {
+                    const int idx = tc_walk(a, w, n_items);
+                    if (idx < 0) break;
+                    const auto it = tc_any_item<Mode>(a, idx, n_qt);
+                    const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
+                    for (int j = 0; j < it.n_kv; ++j, ++t) {
+                        const int s = t % S, k0 = tc_window_key0(it, j);
+                        if (!tc_window_fix(a, it, k0)) continue;
+                        ok = __all_sync(0xffffffffu, tc_wait(v_ask, asked & 1, deadline, abort, a.err, KERR_TIMEOUT_FULL));
+                        if (!ok) break;
+                        ++asked;
+                        for (int r = lane; r < kTcKeys; r += 32) {
+                            const int key = k0 + r;
+                            if (key < it.hi && (key >= it.lo || key < a.sinks)) continue;
+#pragma unroll
+                            for (int c = 0; c < NCH; ++c) {
+                                const uint32_t row = smem_u32(sm + Sm::kV + s * Sm::kKvBytes + c * Sm::kKvChunkBytes + r * 128);
+#pragma unroll
+                                for (int i = 0; i < 128; i += 16) sts128(row + i, 0, 0, 0, 0);
+                            }
+                        }
+                        fence_proxy_async_smem();  // the tensor cores read what these stores wrote
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(v_fixed);
+                    }
+                }
+            }
         } else if (warp == 1 || warp == kTcPvWarp) {
             // ------------------------------------------------------------------ MMA issuers
             // Two issuing threads on different SM sub-partitions: warp 1 issues S = Q.K^T, warp
@@ -573,8 +704,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             // different threads are not ordered, so S(t), which overwrites the S buffer that P(t-2) was
             // packed into, waits for pv_done(t-2).
             if (lane == 0) {
-                constexpr uint32_t kIdS = idesc_bf16(kTcRows, kTcKeys, 0, 0);
-                constexpr uint32_t kIdO = idesc_bf16(kTcRows, D, 0, 1);
+                constexpr uint32_t kIdS = idesc_16bit(kBf16, kTcRows, kTcKeys, 0, 0);
+                constexpr uint32_t kIdO = idesc_16bit(kBf16, kTcRows, D, 0, 1);
                 // Descriptors are built once and advanced by constant offsets: an issuing thread pays
                 // the latency of every instruction between two MMAs.
                 const uint64_t q_desc = smem_desc_sw128(smem_u32(sm + Sm::kQ), 16, 1024);
@@ -584,10 +715,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 bool ok = true;
                 uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
                 int t = 0, z = 0;
+                int asked = 0;  // edge tiles so far
                 for (int w = 0; ok; ++w) {
                     const int idx = tc_walk(a, w, n_items);
                     if (idx < 0) break;
-                    const int n_kv = tc_item(a, idx, n_qt).n_kv;
+                    const auto it = tc_any_item<Mode>(a, idx, n_qt);
+                    const int n_kv = it.n_kv;
                     if (n_kv == 0) continue;
                     deadline = globaltimer_ns() + kWaitLimitNs;
                     const int qb = z & 1, ob = z & 1;
@@ -618,15 +751,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     } else {
                         for (int j = 0; j < n_kv; ++j, ++t) {
                             const int s = t % S, bf = t & 1;
+                            bool fix = false;
+                            if constexpr (kWin) fix = tc_window_fix(a, it, tc_window_key0(it, j));
+                            if (fix) {  // warp 3 zeroes V's unseen rows while the softmax works on the tile
+                                if (!tc_wait(&v_full[s], (t / S) & 1, deadline, abort, a.err, KERR_TIMEOUT_FULL)) {
+                                    ok = false;
+                                    break;
+                                }
+                                mbar_arrive(v_ask);
+                            }
                             // The first P.V of item z overwrites O buffer z & 1: item z - 2's epilogue must
                             // have read it.
                             if ((j == 0 && z >= 2 &&
                                  !tc_wait(&o_free[ob], ((z >> 1) - 1) & 1, deadline, abort, a.err, KERR_TIMEOUT_MMA)) ||
                                 !tc_wait(&p_full[bf], (t >> 1) & 1, deadline, abort, a.err, KERR_TIMEOUT_MMA) ||
-                                !tc_wait(&v_full[s], (t / S) & 1, deadline, abort, a.err, KERR_TIMEOUT_FULL)) {
+                                !tc_wait(&v_full[s], (t / S) & 1, deadline, abort, a.err, KERR_TIMEOUT_FULL) ||
+                                (fix && !tc_wait(v_fixed, asked & 1, deadline, abort, a.err, KERR_TIMEOUT_FULL))) {
                                 ok = false;
                                 break;
                             }
+                            if (fix) ++asked;
                             tc_fence_after();
                             const uint32_t p_tmem = tmem + Tm::kS + bf * kTcKeys;  // P(t) packed in its S buffer
                             const uint32_t o_tmem = tmem + Tm::kO + ob * D;
@@ -671,11 +815,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int w = 0; ok; ++w) {
             const int idx = tc_walk(a, w, n_items);
             if (idx < 0) break;
-            const TcItem it = tc_item(a, idx, n_qt);
+            const auto it = tc_any_item<Mode>(a, idx, n_qt);
             if (it.n_kv == 0) continue;
             const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
             const int qr = it.r0 + row;  // query row within the sequence
             const int r0 = it.r0, kv_len = it.kv_len, n_kv = it.n_kv;
+            int win_p0 = 0;  // position of the tile's first row
+            if constexpr (kWin) win_p0 = it.p0;
             const uint32_t o_tmem = tmem + Tm::kO + (z & 1) * D + lane_off;
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < n_kv; ++j, ++t) {
@@ -686,11 +832,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                                          KERR_TIMEOUT_MMA));
                 if (!ok) break;
                 tc_fence_after();
-                const int k0 = j * kTcKeys;  // key position of column 0 (sequence-relative)
-                const bool edge = (k0 + kTcKeys > kv_len) || (a.causal && k0 + kTcKeys - 1 > a.q_pos0 + r0);
+                int k0 = j * kTcKeys;  // key position of column 0 (sequence-relative)
+                if constexpr (kWin) k0 = tc_window_key0(it, j);
+                const bool edge = kWin ? k0 + kTcKeys > kv_len || k0 + kTcKeys - 1 > win_p0 : (k0 + kTcKeys > kv_len) || (a.causal && k0 + kTcKeys - 1 > a.q_pos0 + r0);
                 // Columns c < lim of this tile are visible to this row (key < kv_len, and key <= the
                 // row's position under the causal mask).
-                const int lim = min(kv_len - k0, a.causal ? a.q_pos0 + qr - k0 + 1 : kTcKeys);
+                const int lim = kWin ? min(kv_len, win_p0 + row + 1) - k0
+                                     : min(kv_len - k0, a.causal ? a.q_pos0 + qr - k0 + 1 : kTcKeys);
                 // The tile's row in registers (one read of TMEM; the softmax warpgroup's register
                 // share holds it), then the row max over 8 independent chains of three-input max.
                 uint32_t r[HK];
@@ -701,6 +849,16 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                     for (int c = 0; c < HK; ++c)
                         if (half * HK + c >= lim) r[c] = __float_as_uint(-INFINITY);
+                if constexpr (kWin) {
+                    // Columns below the row's window and past the first tokens; the last row's window starts
+                    // highest.
+                    if (a.window && k0 < win_p0 + kTcRows - a.window && k0 + kTcKeys > a.sinks) {
+                        const int low = win_p0 + row - a.window + 1 - k0, sink = a.sinks - k0;
+#pragma unroll
+                        for (int c = 0; c < HK; ++c)
+                            if (half * HK + c < low && half * HK + c >= sink) r[c] = __float_as_uint(-INFINITY);
+                    }
+                }
                 float mx8[8];
 #pragma unroll
                 for (int u = 0; u < 8; ++u) mx8[u] = fmaxf(__uint_as_float(r[u]), __uint_as_float(r[8 + u]));
@@ -729,7 +887,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const float mt = mx * c2;
                 const float m_new = (m == -INFINITY || mt > m + 8.0f) ? mt : m;
                 const float ms = m_new == -INFINITY ? 0.f : m_new;
-                const float corr = (m == m_new || m_new == -INFINITY) ? 1.f : fast_exp2(m - m_new);
+                // (Windowed: a row's first tiles may hide all their keys; its O is zero then and needs no rescale.)
+                const float corr = (m == m_new || m_new == -INFINITY || (kWin && m == -INFINITY)) ? 1.f : fast_exp2(m - m_new);
                 m = m_new;
                 // O holds P.V of tiles 0..j-1 of this item once pv_done(t-1) has completed.  It is
                 // waited for only before a rescale (rare).  That wait is exact: the S issuer waited for
@@ -770,7 +929,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                             e.x = fast_exp2(e.x);
                             e.y = fast_exp2(e.y);
                         }
-                        pk[c] = pack_bf16(e.x, e.y);
+                        pk[c] = pack_16bit<typename Mode::Operand>(e.x, e.y);
                         rs4[c & 3] = fadd2(rs4[c & 3], e);
                     }
                     tmem_st32(s_tmem + half * 32, pk);  // P of columns [64h, 64h+64) into [32h, 32h+32)
@@ -810,17 +969,18 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int w = 0; ok; ++w) {
             const int idx = tc_walk(a, w, n_items);
             if (idx < 0) break;
-            const TcItem it = tc_item(a, idx, n_qt);
+            const auto it = tc_any_item<Mode>(a, idx, n_qt);
             const int row0 = it.r0 + quarter * 32;  // first sequence row of this warp's 32 rows
-            float* obase = a.out + ((static_cast<size_t>(it.b) * a.q_seq + row0) * a.q_heads + it.h) * D;
-            const size_t ostride = static_cast<size_t>(a.q_heads) * D;  // floats between rows
+            using Out = typename Mode::Out;
+            Out* obase = (kWin ? static_cast<Out*>(a.wout) : reinterpret_cast<Out*>(a.out)) +
+                         ((static_cast<size_t>(it.b) * a.q_seq + row0) * a.q_heads + it.h) * D;
+            const size_t ostride = static_cast<size_t>(a.q_heads) * D;  // elements between rows
             if (it.n_kv == 0) {  // padded query rows only: zeros, D/4 lanes per row
                 constexpr int F4 = D / 4, RPI = 32 / F4;
 #pragma unroll
                 for (int rr = lane / F4; rr < 32; rr += RPI)
                     if (row0 + rr < a.q_seq)
-                        *reinterpret_cast<float4*>(obase + rr * ostride + 4 * (lane % F4)) =
-                            make_float4(0.f, 0.f, 0.f, 0.f);
+                        tc_store4(obase + rr * ostride + 4 * (lane % F4), make_float4(0.f, 0.f, 0.f, 0.f));
                 continue;
             }
             const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
@@ -829,7 +989,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                                  KERR_TIMEOUT_MMA));
             if (!ok) break;
             // Padded rows (past the valid ones) are written as zeros.
-            const float inv = it.r0 + row < it.nq_valid
+            // So are rows that see no key (windowed form: their sum is zero).
+            const float inv = it.r0 + row < it.nq_valid && (!kWin || lsum[(z % LR) * 2 * kTcRows + row] + lsum[((z % LR) * 2 + 1) * kTcRows + row] != 0.f)
                                   ? 1.0f / (lsum[(z % LR) * 2 * kTcRows + row] + lsum[((z % LR) * 2 + 1) * kTcRows + row])
                                   : 0.f;
             ok = __all_sync(0xffffffffu, tc_wait(&o_final[ob], (z >> 1) & 1, deadline, abort, a.err,
@@ -850,8 +1011,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int k = 0; k < 8; ++k) {
                     const int rr = 4 * k + sub;
                     if (row0 + rr < a.q_seq)
-                        *reinterpret_cast<float4*>(obase + rr * ostride + ch * 32 + 4 * quad) =
-                            *reinterpret_cast<const float4*>(stg + rr * Sm::kStageRow + 4 * quad);
+                        tc_store4(obase + rr * ostride + ch * 32 + 4 * quad,
+                                  *reinterpret_cast<const float4*>(stg + rr * Sm::kStageRow + 4 * quad));
                 }
                 __syncwarp();
             }

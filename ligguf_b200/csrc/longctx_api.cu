@@ -8,6 +8,7 @@
 #include "ligguf_cuda_attn.h"
 #include "api_util.h"
 #include "common.cuh"
+#include "flash_tc.cuh"
 #include "kv4.cuh"
 #include "kv4_decode.cuh"
 #include "rope_rows.cuh"
@@ -18,6 +19,8 @@ using lgapi::fail;
 
 namespace {
 
+// Longest windows, prompts and key ranges of the windowed attention: sums of a few of them stay below 2^31.
+constexpr int kWindowMost = 1 << 28;
 constexpr double kTwoPi = 6.283185307179586476925286766559;
 
 bool type_ok(int t) { return t >= LIGGUF_KV_F32 && t <= LIGGUF_KV_BF16; }
@@ -273,16 +276,84 @@ int kv4_blocks(ligguf_kv4* h, int layer, int seq0, int n_seqs, int pos0, int n, 
     return LIGGUF_ATTN_OK;
 }
 
-template <typename T, typename Out>
-int launch_window_rows(const lg::WindowArgs& a, int D, cudaStream_t st) {
-    const long long blocks = (static_cast<long long>(a.batch) * a.n * a.q_heads + 7) / 8;
-    if (blocks > INT32_MAX) return fail(LIGGUF_ATTN_EUNSUPPORTED, "%d x %d rows in one call", a.batch, a.n);
-    if (D == 64)
-        lg::window_rows_kernel<T, Out, 64><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
-    else
-        lg::window_rows_kernel<T, Out, 128><<<static_cast<unsigned>(blocks), 256, 0, st>>>(a);
-    LG_CUDA(cudaGetLastError());
+// [batch][rows][heads][D] of 16-bit elements; boxes of 64 columns x box_rows rows of one head.
+int make_rows_tmap(CUtensorMap* m, const void* base, bool bf16, int D, int heads, long long stride, int rows, int batch,
+                   long long batch_stride, int box_rows) {
+    auto enc = lgapi::tensor_map_encoder();
+    if (!enc) return fail(LIGGUF_ATTN_ECUDA, "cuTensorMapEncodeTiled is not available from the driver");
+    cuuint64_t dims[4] = {cuuint64_t(D), cuuint64_t(heads), cuuint64_t(rows), cuuint64_t(batch)};
+    cuuint64_t strides[3] = {cuuint64_t(D) * 2, cuuint64_t(stride) * 2, cuuint64_t(batch_stride) * 2};
+    cuuint32_t box[4] = {64u, 1u, cuuint32_t(box_rows), 1u};
+    cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+    const CUresult r = enc(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(base),
+                           dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(LIGGUF_ATTN_EINVAL, "no tensor map for %d rows of stride %lld (%d)", rows, stride, int(r));
     return LIGGUF_ATTN_OK;
+}
+
+template <typename T, typename Out, int D>
+int launch_window_tc(const ligguf_window* h, const lg::WindowArgs& w, cudaStream_t st) {
+    constexpr bool bf16 = lg::KvTraits<T>::kBf16;
+    const int device = h->cfg.device;
+    alignas(64) CUtensorMap tq, tk, tv;
+    int rc;
+    if ((rc = make_rows_tmap(&tq, w.q, bf16, D, w.q_heads, w.q_stride, w.n, w.batch, w.q_batch, lg::kTcRows)) ||
+        (rc = make_rows_tmap(&tk, w.k, bf16, D, w.kv_heads, w.k_stride, w.m, w.batch, w.k_batch, lg::kTcKeys)) ||
+        (rc = make_rows_tmap(&tv, w.v, bf16, D, w.kv_heads, w.v_stride, w.m, w.batch, w.v_batch, lg::kTcKeys)))
+        return rc;
+    auto kern = lg::flash_tc_kernel<D, lg::TcWindow<T, Out>>;
+    static int resident[64] = {};
+    int slots = device < 64 ? resident[device] : 0;
+    if (slots == 0) {
+        LG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lg::TcSmem<D>::kTotal)));
+        // The warpgroups' register shares (setmaxnreg) come out of the registers the CTA launched with.
+        cudaFuncAttributes fa{};
+        LG_CUDA(cudaFuncGetAttributes(&fa, kern));
+        constexpr int need = lg::kTcRegsIssue + 2 * lg::kTcRegsSoftmax + lg::kTcRegsEpilogue;
+        if (fa.numRegs * 4 < need)
+            return fail(LIGGUF_ATTN_ECUDA, "windowed attention kernel built with %d registers per thread, %d needed", fa.numRegs,
+                        (need + 3) / 4);
+        int sms = 0, per_sm = 0;
+        LG_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+        LG_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kern, lg::kTcThreads, lg::TcSmem<D>::kTotal));
+        if (per_sm < 1) return fail(LIGGUF_ATTN_ECUDA, "the windowed attention kernel does not fit on an SM");
+        slots = sms * per_sm;
+        if (device < 64) resident[device] = slots;
+    }
+    lg::TcArgs a = {};
+    a.q_heads = w.q_heads;
+    a.kv_heads = w.kv_heads;
+    a.batch = w.batch;
+    a.q_seq = w.n;
+    a.kv_seq = w.m;
+    a.lens = w.lens;
+    a.causal = 1;
+    a.nrep = w.q_heads / w.kv_heads;
+    a.scale_log2 = w.scale_log2;
+    a.err = h->d_err;
+    a.pos0 = w.pos0;
+    a.window = w.window;
+    a.sinks = w.sinks;
+    a.wout = w.out;
+    const long long items = static_cast<long long>(w.q_heads) * ((w.n + lg::kTcRows - 1) / lg::kTcRows) * w.batch;
+    if (items > INT32_MAX) return fail(LIGGUF_ATTN_EUNSUPPORTED, "%d x %d rows of %d heads in one call", w.batch, w.n, w.q_heads);
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3(static_cast<unsigned>(std::min<long long>(items, slots)));
+    lc.blockDim = dim3(lg::kTcThreads);
+    lc.dynamicSmemBytes = lg::TcSmem<D>::kTotal;
+    lc.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = attr;
+    lc.numAttrs = 1;
+    LG_CUDA(cudaLaunchKernelEx(&lc, kern, tq, tk, tv, a));
+    return LIGGUF_ATTN_OK;
+}
+template <typename T, typename Out>
+int launch_window(const ligguf_window* h, const lg::WindowArgs& a, cudaStream_t st) {
+    return h->cfg.head_dim == 64 ? launch_window_tc<T, Out, 64>(h, a, st) : launch_window_tc<T, Out, 128>(h, a, st);
 }
 
 }  // namespace
@@ -625,7 +696,7 @@ int ligguf_cuda_window_init(const ligguf_window_cfg* cfg, ligguf_window** out) {
     if ((rc = check_heads(c.n_heads, c.n_kv_heads))) return rc;
     if (c.head_dim != 64 && c.head_dim != 128)
         return fail(LIGGUF_ATTN_EUNSUPPORTED, "head_dim %d (supported: 64, 128)", c.head_dim);
-    if (c.window < 0 || c.sinks < 0 || (c.sinks && !c.window))
+    if (c.window < 0 || c.sinks < 0 || c.window > kWindowMost || c.sinks > kWindowMost || (c.sinks && !c.window))
         return fail(LIGGUF_ATTN_EINVAL, "window %d with %d sinks", c.window, c.sinks);
     if (!(c.scale >= 0.f) || std::isinf(c.scale)) return fail(LIGGUF_ATTN_EINVAL, "scale %g", c.scale);
     if (c.in_type != LIGGUF_KV_F16 && c.in_type != LIGGUF_KV_BF16)
@@ -656,12 +727,18 @@ int ligguf_cuda_window_attn_async(ligguf_window* h, int batch, int n, int m, con
                                   const void* d_v, const int* d_pos0, const int* d_lens, void* d_out, void* stream) {
     if (!h) return fail(LIGGUF_ATTN_EINVAL, "null handle");
     const ligguf_window_cfg& c = h->cfg;
-    if (batch < 0 || n < 0 || m < 0) return fail(LIGGUF_ATTN_EINVAL, "batch %d, n %d, m %d", batch, n, m);
+    if (batch < 0 || n < 0 || m < 0 || n > kWindowMost || m > kWindowMost)
+        return fail(LIGGUF_ATTN_EINVAL, "batch %d, n %d, m %d", batch, n, m);
     if (batch == 0 || n == 0) return LIGGUF_ATTN_OK;
     if (!d_q || !d_out || (m && (!d_k || !d_v))) return fail(LIGGUF_ATTN_EINVAL, "null tensor pointer");
     if (!aligned16(d_q) || !aligned16(d_k) || !aligned16(d_v) || !aligned16(d_out))
         return fail(LIGGUF_ATTN_EINVAL, "rows must be 16-byte aligned");
     DeviceGuard dg(c.device);
+    const cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (m == 0) {  // no key to see
+        LG_CUDA(cudaMemsetAsync(d_out, 0, size_t(batch) * n * c.n_heads * c.head_dim * type_size(c.out_type), st));
+        return LIGGUF_ATTN_OK;
+    }
     lg::WindowArgs a = {};
     a.q = d_q;
     a.k = d_k;
@@ -683,12 +760,11 @@ int ligguf_cuda_window_attn_async(ligguf_window* h, int batch, int n, int m, con
     a.window = c.window;
     a.sinks = c.sinks;
     a.scale_log2 = c.scale * 1.4426950408889634f;
-    const cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (c.in_type == LIGGUF_KV_F16)
-        return c.out_type == LIGGUF_KV_F32 ? launch_window_rows<__half, float>(a, c.head_dim, st)
-                                           : launch_window_rows<__half, __half>(a, c.head_dim, st);
-    return c.out_type == LIGGUF_KV_F32 ? launch_window_rows<__nv_bfloat16, float>(a, c.head_dim, st)
-                                       : launch_window_rows<__nv_bfloat16, __nv_bfloat16>(a, c.head_dim, st);
+        return c.out_type == LIGGUF_KV_F32 ? launch_window<__half, float>(h, a, st)
+                                           : launch_window<__half, __half>(h, a, st);
+    return c.out_type == LIGGUF_KV_F32 ? launch_window<__nv_bfloat16, float>(h, a, st)
+                                       : launch_window<__nv_bfloat16, __nv_bfloat16>(h, a, st);
 }
 
 int ligguf_cuda_window_status(ligguf_window* h, void* stream) {
