@@ -7,10 +7,15 @@
 // Bound by the cache's bytes (18 D a tile of 16 positions and KV head) as long as the arithmetic on them
 // stays short, so both products run on the tensor cores (mma.m16n8k16, fp16 operands, fp32 sums) straight
 // from the packed codes:
-//   - A code n (0..15) masked into the low mantissa bits of a half is the subnormal n * 2^-24, and shifted
-//     by a nibble n * 2^-20: exact operands that cost one AND for two codes.  The powers of two are taken
-//     out of the fp32 results; the -8 of (n - 8) d enters as the products' initial value (keys) or is
-//     subtracted once at the end (values).
+//   - Keys: a code n (0..15) masked into the low mantissa bits of a half is the subnormal n * 2^-24, and
+//     shifted by a nibble n * 2^-20: exact operands that cost one AND for two codes.  The powers of two are
+//     taken out of the fp32 results, and the -8 of (n - 8) d enters as the products' initial value.  The
+//     tensor cores align products by their operands' exponent fields and cut off what lies 24 bits below the
+//     largest, and a subnormal's field is that of 2^-14: so the queries' hi parts are whole numbers, which
+//     makes every product and sum of hi parts exact, cut or not.
+//   - Values: the weights cannot be whole numbers, and with subnormal codes that cut costs 7 bits (results
+//     were off by 9e-6).  So 0x6400 is OR-ed in by the same instruction (1024 + n, or 1024 + 16 n), and one
+//     packed subtraction (or multiply-add) makes it n - 8: normal halves, exact as well.
 //   - S^T = K Q^T: 16 positions x 8 columns.  The key scales multiply the fp32 sums of their 32 elements.
 //   - Queries and weights are split into two halves each, hi + lo, which together hold 22 bits, so the
 //     results are those of fp32 arithmetic.  Up to four query heads a KV head share one product: columns
@@ -77,16 +82,15 @@ struct Kv4DecodeSmem {
     static constexpr int kRow = D + 8;                // floats of a head's row of kO: two heads apart, other banks
     static constexpr size_t kRing = 0;
     static constexpr size_t kFrag = kRing + size_t(kKv4Warps) * kStages * 2 * Kv4<D>::kTileBytes;  // [kParts][D/16][32] uint2
-    static constexpr size_t kSum = kFrag + size_t(kParts) * (D / 16) * 32 * 8;                     // [8][D/32]
-    static constexpr size_t kScale = kSum + 8 * (D / 32) * 4;                                      // [8]
+    static constexpr size_t kSum = kFrag + size_t(kParts) * (D / 16) * 32 * 8;                     // [kParts * 8][D/32]
+    static constexpr size_t kScale = kSum + size_t(kParts) * 8 * (D / 32) * 4;                     // [8]
     static constexpr size_t kQ = kScale + 8 * 4;
     static constexpr size_t kGamma = kQ + NREP * D * 4;  // norm weights of q and k
     static constexpr size_t kKn = kGamma + 2 * D * 4;
     static constexpr size_t kVn = kKn + D * 4;
     static constexpr size_t kCs = kVn + D * 4;
     static constexpr size_t kO = kCs + D / 2 * 8;                             // [warps][NREP][kRow]
-    static constexpr size_t kW = kO + size_t(kKv4Warps) * NREP * kRow * 4;    // [warps][NREP][D/32]
-    static constexpr size_t kM = kW + size_t(kKv4Warps) * NREP * (D / 32) * 4;  // [warps + 1][NREP]
+    static constexpr size_t kM = kO + size_t(kKv4Warps) * NREP * kRow * 4;    // [warps + 1][NREP]
     static constexpr size_t kL = kM + (kKv4Warps + 1) * NREP * 4;
     static constexpr size_t kJoin = (kL + (kKv4Warps + 1) * NREP * 4 + 15) / 16 * 16;  // sums of a join's groups
     static constexpr size_t kBar = kJoin + kKv4Threads * 16;
@@ -256,6 +260,18 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     return r;
 }
 __device__ __forceinline__ float2 unpack_f16(uint32_t x) { return __half22float2(*reinterpret_cast<const __half2*>(&x)); }
+// n - 8 for the codes in bits 0-3 (code_low) or 4-7 (code_high) of both 16-bit halves, as halves.
+__device__ __forceinline__ uint32_t code_low(uint32_t w) {
+    const uint32_t x = (w & 0x000F000Fu) | 0x64006400u;
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(1032.f, 1032.f));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+__device__ __forceinline__ uint32_t code_high(uint32_t w) {
+    const uint32_t x = (w & 0x00F000F0u) | 0x64006400u;
+    const __half2 d = __hfma2(*reinterpret_cast<const __half2*>(&x), __floats2half2_rn(0.0625f, 0.0625f),
+                              __floats2half2_rn(-72.f, -72.f));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -289,10 +305,13 @@ __device__ __forceinline__ void kv4_query_operands(const float (&x)[8], int head
     float sh = 0.f, sl = 0.f;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-        const float d0 = x[4 * u] * up, d1 = x[4 * u + 1] * up * 0.0625f, d2 = x[4 * u + 2] * up, d3 = x[4 * u + 3] * up * 0.0625f;
-        const uint2 hi = make_uint2(pack_f16(d0, d2), pack_f16(d1, d3));
-        const float2 h0 = unpack_f16(hi.x), h1 = unpack_f16(hi.y);
-        const uint2 lo = make_uint2(pack_f16(d0 - h0.x, d2 - h0.y), pack_f16(d1 - h1.x, d3 - h1.y));
+        // hi: whole numbers, so that every product with a code and every sum of a group's is exact; lo: what is
+        // left, at most a half.
+        const float v0 = x[4 * u] * up, v1 = x[4 * u + 1] * up, v2 = x[4 * u + 2] * up, v3 = x[4 * u + 3] * up;
+        const float w0 = rintf(v0), w1 = rintf(v1), w2 = rintf(v2), w3 = rintf(v3);
+        const uint2 hi = make_uint2(pack_f16(w0, w2), pack_f16(w1 * 0.0625f, w3 * 0.0625f));
+        const uint2 lo = make_uint2(pack_f16(v0 - w0, v2 - w2), pack_f16((v1 - w1) * 0.0625f, (v3 - w3) * 0.0625f));
+        const float2 h0 = make_float2(w0, w2), h1 = make_float2(w1 * 0.0625f, w3 * 0.0625f);
         const float2 r0 = unpack_f16(lo.x), r1 = unpack_f16(lo.y);
         sh += (h0.x + h0.y) + 16.f * (h1.x + h1.y);
         sl += (r0.x + r0.y) + 16.f * (r1.x + r1.y);
@@ -309,12 +328,8 @@ __device__ __forceinline__ void kv4_query_operands(const float (&x)[8], int head
     }
     constexpr float k8 = -8.f / 16777216.f;
     if (lane < L && (l & 3) == 0) {
-        if (kWide) {
-            sums[head * G + (l >> 2)] = k8 * (sh + sl);
-        } else {
-            sums[head * G + (l >> 2)] = k8 * sh;
-            sums[(4 + head) * G + (l >> 2)] = k8 * sl;
-        }
+        sums[head * G + (l >> 2)] = k8 * sh;
+        sums[((kWide ? 8 : 4) + head) * G + (l >> 2)] = k8 * sl;
     }
     if (lane == 0) {
         const float down = __int_as_float((127 + e + 14) << 23);  // 2^(e - 10) * 2^24
@@ -353,9 +368,9 @@ struct Kv4Warp {
     static constexpr bool kWide = NREP > 4;  // hi and lo parts as two products
     static constexpr int KS = D / 16, G = D / 32;
     uint32_t b[kWide ? 2 : 1][KS][2];  // queries, as B operands
-    float c[G][2];                     // -8 * sum of a group's queries, of this lane's columns
+    float c[kWide ? 2 : 1][G][2];      // -8 * sum of a group's queries, of this lane's columns
     float sx[2];                       // scales of the scores of this lane's two heads
-    float m[2], l[2], ws[G][2];        // running maxima, sums of weights and of weights * value scales
+    float m[2], l[2];                  // running maxima and sums of weights
     float o[KS][4];
 
     // From what kv4_query_operands left in shared memory.
@@ -369,15 +384,15 @@ struct Kv4Warp {
                 b[p][j][0] = f.x, b[p][j][1] = f.y;
             }
 #pragma unroll
-        for (int i = 0; i < G; ++i) {
-            c[i][0] = sums[2 * t * G + i];
-            c[i][1] = sums[(2 * t + 1) * G + i];
-        }
+        for (int p = 0; p < (kWide ? 2 : 1); ++p)
+#pragma unroll
+            for (int i = 0; i < G; ++i) {
+                c[p][i][0] = sums[(8 * p + 2 * t) * G + i];
+                c[p][i][1] = sums[(8 * p + 2 * t + 1) * G + i];
+            }
         sx[0] = scales[2 * t], sx[1] = scales[2 * t + 1];
 #pragma unroll
         for (int i = 0; i < 2; ++i) m[i] = -1e30f, l[i] = 0.f;
-#pragma unroll
-        for (int i = 0; i < G; ++i) ws[i][0] = ws[i][1] = 0.f;
 #pragma unroll
         for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     }
@@ -394,15 +409,18 @@ struct Kv4Warp {
 #pragma unroll
             for (int gr = 0; gr < 2; ++gr) {
                 const int i = ch * 2 + gr;
-                float s[4] = {c[i][0], c[i][1], c[i][0], c[i][1]};
+                float s[4] = {c[0][i][0], c[0][i][1], c[0][i][0], c[0][i][1]}, s2[4];
+                if constexpr (kWide)  // sums of their own: added to those of the hi parts they would be cut off
+                    s2[0] = s2[2] = c[1][i][0], s2[1] = s2[3] = c[1][i][1];
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int j = 2 * i + u;
                     const uint32_t lo = w[2 * gr + u], hi = lo >> 8;
                     const uint32_t a0 = lo & 0x000F000Fu, a2 = lo & 0x00F000F0u, a1 = hi & 0x000F000Fu, a3 = hi & 0x00F000F0u;
                     mma_f16(s, a0, a1, a2, a3, b[0][j][0], b[0][j][1], s[0], s[1], s[2], s[3]);
-                    if constexpr (kWide) mma_f16(s, a0, a1, a2, a3, b[1][j][0], b[1][j][1], s[0], s[1], s[2], s[3]);
+                    if constexpr (kWide) mma_f16(s2, a0, a1, a2, a3, b[1][j][0], b[1][j][1], s2[0], s2[1], s2[2], s2[3]);
                 }
+                if constexpr (kWide) s[0] += s2[0], s[1] += s2[1], s[2] += s2[2], s[3] += s2[3];
                 x[0] = fmaf(s[0], ks[0][i], x[0]);
                 x[1] = fmaf(s[1], ks[0][i], x[1]);
                 x[2] = fmaf(s[2], ks[1][i], x[2]);
@@ -440,8 +458,7 @@ struct Kv4Warp {
     // O += V^T W for one word of the value codes (16 elements of the head).
     __device__ __forceinline__ void values(uint32_t lo, int j, uint32_t b0, uint32_t b1) {
         const uint32_t hi = lo >> 8;
-        mma_f16(o[j], lo & 0x000F000Fu, lo & 0x00F000F0u, hi & 0x000F000Fu, hi & 0x00F000F0u, b0, b1, o[j][0], o[j][1], o[j][2],
-                o[j][3]);
+        mma_f16(o[j], code_low(lo), code_high(lo), code_low(hi), code_high(hi), b0, b1, o[j][0], o[j][1], o[j][2], o[j][3]);
     }
     __device__ __forceinline__ static bool edge(const Kv4Row& r, int k0) { return k0 + kKv4Tile > r.pos || k0 < r.first; }
 
@@ -514,8 +531,6 @@ struct Kv4Warp {
     __device__ __forceinline__ void split(int i, const float (&p)[4], const float (&vs)[2][G], uint32_t& h0, uint32_t& h1,
                                           uint32_t& l0, uint32_t& l1) {
         const float v0 = p[0] * vs[0][i], v1 = p[1] * vs[0][i], v2 = p[2] * vs[1][i], v3 = p[3] * vs[1][i];
-        ws[i][0] += v0 + v2;
-        ws[i][1] += v1 + v3;
         h0 = pack_f16(v0, v1);
         h1 = pack_f16(v2, v3);
         const float2 f0 = unpack_f16(h0), f1 = unpack_f16(h1);
@@ -534,8 +549,6 @@ struct Kv4Warp {
         const float f0 = ex2(m[0] - n0), f1 = ex2(m[1] - n1);
         m[0] = n0, m[1] = n1;
         l[0] *= f0, l[1] *= f1;
-#pragma unroll
-        for (int i = 0; i < G; ++i) ws[i][0] *= f0, ws[i][1] *= f1;
 #pragma unroll
         for (int j = 0; j < KS; ++j) o[j][0] *= f0, o[j][1] *= f1, o[j][2] *= f0, o[j][3] *= f1;
     }
@@ -576,33 +589,28 @@ struct Kv4Warp {
         return make_float2(e[0], e[1]);
     }
 
-    // Sums over the warp's rows, to shared memory: o [NREP][kRow] short of -8 times sw [NREP][G], m and l
-    // [NREP]; all relative to 2^m.
-    __device__ __forceinline__ void finish(float* so, float* sw, float* sm, float* sl, int lane) {
+    // Sums over the warp's rows, to shared memory: o [NREP][kRow], m and l [NREP]; all relative to 2^m.
+    __device__ __forceinline__ void finish(float* so, float* sm, float* sl, int lane) {
         constexpr int kRow = Kv4DecodeSmem<D, NREP>::kRow;
         const int g = lane >> 2, t = lane & 3;
         const int h0 = kWide ? 2 * t : 2 * (t & 1);  // this lane's columns are heads h0, h0 + 1
         const bool first = kWide || t < 2;
-        float wv[2 * G], lv[2] = {l[0], l[1]};
-#pragma unroll
-        for (int i = 0; i < G; ++i) wv[2 * i] = ws[i][0], wv[2 * i + 1] = ws[i][1];
-        const float w = rows_sum<2 * G, !kWide>(wv, lane), ls = rows_sum<2, !kWide>(lv, lane);
-        const int wi = rows_value<2 * G>(lane), li = rows_value<2>(lane);
-        if (first && h0 + (wi & 1) < NREP) sw[(h0 + (wi & 1)) * G + (wi >> 1)] = 8.f * w;
+        float lv[2] = {l[0], l[1]};
+        const float ls = rows_sum<2, !kWide>(lv, lane);
+        const int li = rows_value<2>(lane);
         if (first && h0 + li < NREP) sl[h0 + li] = ls, sm[h0 + li] = (li ? m[1] : m[0]) - 7.f;
-        // Rows g and g + 8 of k-step j are elements 16j + 2g, 16j + 2g + 1; their sums are short of 2^24, 2^20.
+        // Rows g and g + 8 of k-step j are elements 16j + 2g, 16j + 2g + 1.
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
             float* at = so + h0 * kRow + 16 * j + 2 * g;
             if constexpr (kWide) {
-                *reinterpret_cast<float2*>(at) = make_float2(o[j][0] * 16777216.f, o[j][2] * 1048576.f);
-                *reinterpret_cast<float2*>(at + kRow) = make_float2(o[j][1] * 16777216.f, o[j][3] * 1048576.f);
+                *reinterpret_cast<float2*>(at) = make_float2(o[j][0], o[j][2]);
+                *reinterpret_cast<float2*>(at + kRow) = make_float2(o[j][1], o[j][3]);
             } else {  // hi and lo columns lie two lanes apart: one lane adds rows g, the other rows g + 8
                 const float y0 = (first ? o[j][0] : o[j][2]) + __shfl_xor_sync(0xffffffffu, first ? o[j][2] : o[j][0], 2);
                 const float y1 = (first ? o[j][1] : o[j][3]) + __shfl_xor_sync(0xffffffffu, first ? o[j][3] : o[j][1], 2);
-                const float f = first ? 16777216.f : 1048576.f;
-                if (h0 < NREP) at[first ? 0 : 1] = y0 * f;
-                if (h0 + 1 < NREP) at[kRow + (first ? 0 : 1)] = y1 * f;
+                if (h0 < NREP) at[first ? 0 : 1] = y0;
+                if (h0 + 1 < NREP) at[kRow + (first ? 0 : 1)] = y1;
             }
         }
     }
@@ -624,7 +632,6 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
     float* so = reinterpret_cast<float*>(smem + Sm::kO);
     float* sm = reinterpret_cast<float*>(smem + Sm::kM);
     float* sl = reinterpret_cast<float*>(smem + Sm::kL);
-    float* sw = reinterpret_cast<float*>(smem + Sm::kW);
     volatile int* abort = reinterpret_cast<volatile int*>(smem + Sm::kMisc);
     int* last = reinterpret_cast<int*>(smem + Sm::kMisc + 4);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -798,7 +805,7 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
             ++taken;
             fill();
         }
-        acc.finish(so + warp * NREP * Sm::kRow, sw + warp * NREP * (D / 32), sm + warp * NREP, sl + warp * NREP, lane);
+        acc.finish(so + warp * NREP * Sm::kRow, sm + warp * NREP, sl + warp * NREP, lane);
         if (own)  // the token itself: one key whose weight is 1 relative to its own score
             for (int h = warp; h < NREP; h += kKv4Warps) {
                 float x = 0.f;
@@ -824,7 +831,7 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
             for (int w = 0; w < kKv4Warps; ++w) {
                 const float f = ex2(mw[w] - M);
                 lsum = fmaf(sl[w * NREP + h], f, lsum);
-                osum = fmaf(so[(w * NREP + h) * Sm::kRow + d] - sw[(w * NREP + h) * (D / 32) + d / 32], f, osum);
+                osum = fmaf(so[(w * NREP + h) * Sm::kRow + d], f, osum);
             }
             if (whole) {
                 out[i] = KvTraits<In>::from_float(osum / lsum);

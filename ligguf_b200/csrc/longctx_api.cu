@@ -105,14 +105,23 @@ int rope_layout(const ligguf_rope_cfg& r) {
 template <typename In, typename Out, int D>
 int launch_rope_rows(lg::RopeRowsArgs& a, int layout, cudaStream_t st) {
     const int units = ((a.q ? a.q_heads : 0) + a.kv_heads * (a.v ? 2 : 1)) * (D / 8);
-    a.units_per_block = a.n >= 256 ? (units + 255) / 256 * 256 : 256;
+    // Many tokens: a block a token, whose threads take kRopeAhead units each.  Few: a unit a thread, the
+    // token's heads over several blocks (each computes the rotation again, which takes less than a block's
+    // units one after another).
+    int threads = 128;
+    if (a.n >= 256) {
+        threads = std::min(256, (units + 32 * lg::kRopeAhead - 1) / (32 * lg::kRopeAhead) * 32);
+        a.units_per_block = (units + 31) / 32 * 32;
+    } else {
+        a.units_per_block = threads;
+    }
     const dim3 grid(a.n, (units + a.units_per_block - 1) / a.units_per_block);
     if (layout == lg::kRopeAdjacent)
-        lg::rope_rows_kernel<In, Out, D, lg::kRopeAdjacent><<<grid, 256, 0, st>>>(a);
+        lg::rope_rows_kernel<In, Out, D, lg::kRopeAdjacent><<<grid, threads, 0, st>>>(a);
     else if (layout == lg::kRopeHalves)
-        lg::rope_rows_kernel<In, Out, D, lg::kRopeHalves><<<grid, 256, 0, st>>>(a);
+        lg::rope_rows_kernel<In, Out, D, lg::kRopeHalves><<<grid, threads, 0, st>>>(a);
     else
-        lg::rope_rows_kernel<In, Out, D, lg::kRopeHalvesOdd><<<grid, 256, 0, st>>>(a);
+        lg::rope_rows_kernel<In, Out, D, lg::kRopeHalvesOdd><<<grid, threads, 0, st>>>(a);
     LG_CUDA(cudaGetLastError());
     return LIGGUF_ATTN_OK;
 }

@@ -341,6 +341,22 @@ def test_kv4_decode_value_magnitudes(gpu, spread):
     close(out, want, 2e-5 * np.abs(want).max())
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("nrep", [1, 2, 4, 8])
+@pytest.mark.parametrize("n", [15, 600, 5000])
+def test_kv4_decode_holds_fp32_accuracy_with_unlike_weights(gpu, dim, nrep, n):
+    """Scores spread over twenty powers of two: the halves that the tensor cores multiply together hold the
+    queries and the weights to 2^-22, so the relative error (2-norm) stays within that of fp32 scores of this
+    size: 20 * 2^-24 * ln 2 a weight, and as much again for the sums: 2e-6."""
+    rng = np.random.default_rng(n + nrep)
+    c = make_cache(dim, 2, nrep, n_context=n + 1, rope_dim=0)
+    kb, vb, qkv, d = decode_case(rng, c, [n], F32)
+    q = (qkv[0] * 3).astype(np.float32)
+    out, _, _ = run_decode(c, (dev(q), d[1], d[2]), [n], F32)
+    want = decode_ref(c, kb, vb, (q, qkv[1], qkv[2]), [n])
+    assert np.linalg.norm(out - want) <= 2e-6 * np.linalg.norm(want)
+
+
 def test_kv4_decode_mixed_value_magnitudes_and_large_scores(gpu):
     """Keys of very different scores and rows of very different values: a row of large values that gets a
     tiny weight, and one of tiny values that gets nearly all."""
