@@ -31,6 +31,8 @@ struct RopeRowsArgs {
     uint8_t* tiles;  // first tile of (layer, sequence, head 0)
     long long tiles_per_head;
     void *k_rows, *v_rows;  // the rows as the cache holds them, or null
+    int kv_heads_per_block; // of a block that takes tiles of keys and values
+    int parts;              // blocks of a token, and the units of each
     int units_per_block;
 };
 
@@ -164,23 +166,230 @@ __device__ __forceinline__ void rope_rows_unit(const RopeRowsArgs& a, long long 
     }
 }
 
-// Block (token, part of its units): a token's rotation is computed once for all its heads, with the first
-// kRopeAhead units of every thread already in flight.
-constexpr int kRopeAhead = 4;
+// Two units of a head that one thread takes together: the halves of eight rotated pairs (or, past the rotated
+// part and for adjacent pairs, neighbours), so a rotation needs no exchange and reads its table once.
+template <int D, int kLayout>
+__device__ __forceinline__ int2 rope_two_units(int dl, int pairs) {
+    if (kLayout == kRopeHalves) {
+        const int hl = pairs / 8;
+        if (dl < hl) return make_int2(dl, dl + hl);
+    }
+    return make_int2(2 * dl, 2 * dl + 1);  // (past the rotated part: 2 hl + 2 (dl - hl))
+}
+
+// A prompt's keys and values: block (tile of 16 positions, a few KV heads).  A thread holds 8 elements of one
+// position, the same of every head, so it forms its rotations once; a head's codes are put together in shared
+// memory and leave as whole 16-byte words (byte by byte they cost more than the rest of the kernel).  Positions
+// of the tile outside the prompt keep their bytes: such tiles are written byte by byte.
+constexpr int kKv4AppendBlocks = 3;  // resident on an SM
+constexpr int kRopePairRow = 64 + 8;  // table entries of a position: two positions of a warp in other banks
+template <typename In, typename Out, int D, int kLayout>
+__global__ void __launch_bounds__(256, kKv4AppendBlocks) kv4_append_kernel(const RopeRowsArgs a) {
+    constexpr int L = D / 8, kHeads = 256 / (16 * L), TB = Kv4<D>::kTileBytes;  // heads at a time
+    __shared__ float2 cs[16 * kRopePairRow];
+    __shared__ uint4 staging[kHeads * TB / 16];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the queries' kernel needs nothing of this one's
+    const int block = blockIdx.x;
+    const int groups = (a.kv_heads + a.kv_heads_per_block - 1) / a.kv_heads_per_block;
+    const int t0 = a.pos0 / kKv4Tile * kKv4Tile + block / groups * kKv4Tile;
+    const int h0 = block % groups * a.kv_heads_per_block, h1 = min(a.kv_heads, h0 + a.kv_heads_per_block);
+    const int l = threadIdx.x % L, p = threadIdx.x / L % 16, sub = threadIdx.x / (16 * L);
+    const int pos = t0 + p;
+    const bool live = pos >= a.pos0 && pos < a.pos0 + a.n;
+    const bool whole = t0 >= a.pos0 && t0 + kKv4Tile <= a.pos0 + a.n;
+    const long long tok = pos - a.pos0;
+    Units<In> k, v;
+    auto load = [&](int h) {
+        if (live && h < h1) {
+            k.load(static_cast<const In*>(a.k) + tok * a.k_stride + h * D + l * 8);
+            v.load(static_cast<const In*>(a.v) + tok * a.v_stride + h * D + l * 8);
+        } else {
+            k.zero();
+            v.zero();
+        }
+    };
+    load(h0 + sub);
+    for (int i = threadIdx.x; i < 16 * a.pairs; i += 256)
+        cs[i / a.pairs * kRopePairRow + rope_slot<kLayout>(i % a.pairs)] = rope_turn(a.turns[i % a.pairs], t0 + i / a.pairs, a.magnitude);
+    __syncthreads();
+    // This thread's rotations: of its four pairs, or of the eight pairs it has a half of.
+    constexpr int kTurns = kLayout == kRopeAdjacent ? 4 : 8;
+    float2 w[kTurns];
+    const int hl = a.pairs / 8;
+    const bool low = l < hl;
+#pragma unroll
+    for (int i = 0; i < kTurns; ++i) {
+        const int pair = kLayout == kRopeAdjacent ? 4 * l + i : 8 * (low ? l : l - hl) + i;
+        w[i] = (kLayout == kRopeAdjacent ? pair < a.pairs : l < 2 * hl) ? cs[p * kRopePairRow + rope_slot<kLayout>(pair)] : make_float2(1.f, 0.f);
+    }
+    float g[8];
+    if (a.norm) load8(a.k_gamma + l * 8, g);
+    uint8_t* stage = reinterpret_cast<uint8_t*>(staging) + sub * TB;
+    for (int h = h0 + sub; h - sub < h1; h += kHeads) {
+        float x[8], y[8];
+        k.get(x);
+        v.get(y);
+        load(h + kHeads);
+        if (a.norm) {
+            float ss = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+            const float rs = rsqrtf(head_sum<L>(ss) * (1.0f / D) + a.eps);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = (x[i] * rs) * g[i];
+        }
+        if constexpr (kLayout == kRopeAdjacent) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x0 = x[2 * i], x1 = x[2 * i + 1];
+                x[2 * i] = x0 * w[i].x - x1 * w[i].y;
+                x[2 * i + 1] = x0 * w[i].y + x1 * w[i].x;
+            }
+        } else {
+            const int from = (low ? l + hl : l < 2 * hl ? l - hl : l) & (L - 1);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float other = __shfl_sync(0xffffffffu, x[i], from, L);
+                x[i] = x[i] * w[i].x + (low ? -other : other) * w[i].y;
+            }
+        }
+        uint32_t kc, vc;
+        const __half kd = kv4_quantize8(x, kc), vd = kv4_quantize8(y, vc);
+        uint8_t* tile = a.tiles + (h * a.tiles_per_head + t0 / kKv4Tile) * TB;
+        const bool on = live && h < h1;
+        if (on) {
+            uint8_t* dst = whole ? stage : tile;
+            kv4_store8<D, false>(dst, p, l, kc, kd);
+            kv4_store8<D, true>(dst, p, l, vc, vd);
+        }
+        if (whole) {
+            __syncthreads();
+            if (h < h1)
+                for (int i = threadIdx.x % (16 * L); i < TB / 16; i += 16 * L)
+                    reinterpret_cast<uint4*>(tile)[i] = reinterpret_cast<const uint4*>(stage)[i];
+        }
+        if (on && a.k_rows) {
+            float z[8];
+            kv4_values8(kc, kd, z);
+            store8(static_cast<Out*>(a.k_rows) + (tok * a.kv_heads + h) * D + l * 8, z);
+        }
+        if (on && a.v_rows) {
+            float z[8];
+            kv4_values8(vc, vd, z);
+            store8(static_cast<Out*>(a.v_rows) + (tok * a.kv_heads + h) * D + l * 8, z);
+        }
+        if (whole) __syncthreads();
+    }
+}
+
+// One head's two units in p and r: norm, rotation.  Lanes of D/16 hold a head.
+template <int D, int kLayout>
+__device__ __forceinline__ void rope_two(const RopeRowsArgs& a, const float* gamma, int dl, int2 two, const float2* cs,
+                                         float (&p)[8], float (&r)[8]) {
+    if (a.norm) {
+        float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s0 = fmaf(p[i], p[i], s0), s1 = fmaf(r[i], r[i], s1);
+        const float rs = rsqrtf(head_sum<D / 16>(s0 + s1) * (1.0f / D) + a.eps);
+        float g[8];
+        load8(gamma + two.x * 8, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) p[i] = (p[i] * rs) * g[i];
+        load8(gamma + two.y * 8, g);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = (r[i] * rs) * g[i];
+    }
+    if constexpr (kLayout == kRopeHalves) {
+        if (dl < a.pairs / 8)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float2 w = cs[rope_slot<kLayout>(8 * dl + i)];
+                const float x0 = p[i], x1 = r[i];
+                p[i] = x0 * w.x - x1 * w.y;
+                r[i] = x0 * w.y + x1 * w.x;
+            }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float* z = i < 4 ? p + 2 * i : r + 2 * (i - 4);
+            if (8 * dl + i < a.pairs) {
+                const float2 w = cs[rope_slot<kLayout>(8 * dl + i)];
+                const float x0 = z[0], x1 = z[1];
+                z[0] = x0 * w.x - x1 * w.y;
+                z[1] = x0 * w.y + x1 * w.x;
+            }
+        }
+    }
+}
+
+// Heads that are only normed and rotated, a block a token, by pairs of units; a thread takes the same pair of
+// every head it takes.
+template <typename In, typename Out, int D, int kLayout>
+__global__ void __launch_bounds__(256) rope_pairs_kernel(const RopeRowsArgs a) {
+    constexpr int DL = D / 16, kTake = sizeof(In) == 4 ? 1 : 2;  // heads of a thread at a time
+    __shared__ float2 cs[64];
+    const int qh = a.q ? a.q_heads : 0, heads = qh + (a.tiles ? 0 : a.kv_heads);
+    const int dl = threadIdx.x % DL, step = blockDim.x / DL, h0 = threadIdx.x / DL;
+    const int2 two = rope_two_units<D, kLayout>(dl, a.pairs);
+    const long long tok = blockIdx.x;
+    Units<In> x[2 * kTake];
+    auto load = [&](int h) {
+#pragma unroll
+        for (int n = 0; n < kTake; ++n, h += step) {
+            if (h < heads) {
+                const In* src = h < qh ? static_cast<const In*>(a.q) + tok * a.q_stride + h * D
+                                       : static_cast<const In*>(a.k) + tok * a.k_stride + (h - qh) * D;
+                x[2 * n].load(src + two.x * 8);
+                x[2 * n + 1].load(src + two.y * 8);
+            } else {
+                x[2 * n].zero();
+                x[2 * n + 1].zero();
+            }
+        }
+    };
+    load(h0);
+    const int pos = a.pos ? a.pos[tok] : a.pos0 + static_cast<int>(tok);
+    for (int i = threadIdx.x; i < a.pairs; i += blockDim.x)
+        cs[rope_slot<kLayout>(i)] = rope_turn(a.turns[i], pos, a.magnitude);
+    __syncthreads();
+    for (int h = h0; h - h0 < heads; h += kTake * step) {
+        if (h != h0) load(h);
+#pragma unroll
+        for (int n = 0; n < kTake; ++n) {
+            const int hn = h + n * step;
+            float p[8], r[8];
+            x[2 * n].get(p);
+            x[2 * n + 1].get(r);
+            rope_two<D, kLayout>(a, hn < qh ? a.q_gamma : a.k_gamma, dl, two, cs, p, r);
+            if (hn < heads) {
+                Out* dst = hn < qh ? static_cast<Out*>(a.q_out) + tok * a.q_out_stride + hn * D
+                                   : static_cast<Out*>(a.k_out) + tok * a.k_out_stride + (hn - qh) * D;
+                store8(dst + two.x * 8, p);
+                store8(dst + two.y * 8, r);
+            }
+        }
+    }
+    // Launched beside kv4_append_kernel, whose completion this grid's stands for.
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
+// Block (token, part of its units), a unit a thread: few tokens, and halves that are not whole units apart.  A
+// token's rotation is computed once for the block's heads, with its first loads already in flight.
+constexpr int kRopeAhead = 4;  // units a thread has in flight
 template <typename In, typename Out, int D, int kLayout>
 __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeRowsArgs a) {
     constexpr int L = D / 8;  // units (lanes) of a head
     __shared__ float2 cs[64];
     __shared__ float xch[kLayout == kRopeHalvesOdd ? 256 * 8 : 1];
-    const long long tok = blockIdx.x;
+    const int part = blockIdx.x % a.parts;
+    const long long tok = blockIdx.x / a.parts;
     const int q_units = a.q ? a.q_heads * L : 0, k_units = a.kv_heads * L;
-    const int total = q_units + k_units + (a.v ? k_units : 0);
-    const int u1 = min(total, static_cast<int>(blockIdx.y + 1) * a.units_per_block);
     const int pos = a.pos ? a.pos[tok] : a.pos0 + static_cast<int>(tok);
+    const int u1 = min(q_units + k_units + (a.v ? k_units : 0), (part + 1) * a.units_per_block);
     const int lane = threadIdx.x & 31;
     bool first = true;
     // Whole warps stay together: the shuffles below need every lane (units past the end work on zeros).
-    for (int u0 = blockIdx.y * a.units_per_block + (threadIdx.x & ~31); first || u0 < u1; u0 += kRopeAhead * blockDim.x) {
+    for (int u0 = part * a.units_per_block + static_cast<int>(threadIdx.x & ~31); first || u0 < u1; u0 += kRopeAhead * blockDim.x) {
         Units<In> x[kRopeAhead];
 #pragma unroll
         for (int n = 0; n < kRopeAhead; ++n) {
@@ -199,8 +408,8 @@ __global__ void __launch_bounds__(256) rope_rows_kernel(const RopeRowsArgs a) {
             for (int i = threadIdx.x; i < a.pairs; i += blockDim.x)
                 cs[rope_slot<kLayout>(i)] = rope_turn(a.turns[i], pos, a.magnitude);
             __syncthreads();
-            first = false;
         }
+        first = false;
 #pragma unroll
         for (int n = 0; n < kRopeAhead; ++n) {
             const int u = u0 + n * blockDim.x + lane;
