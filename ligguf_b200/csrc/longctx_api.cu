@@ -220,6 +220,8 @@ struct ligguf_kv4 {
 
 struct ligguf_window {
     ligguf_window_cfg cfg;
+    float* parts = nullptr;  // few rows: partial sums of the splits
+    int num_sms = 0;
     int *h_err = nullptr, *d_err = nullptr;
 };
 
@@ -396,9 +398,66 @@ int launch_window_tc(const ligguf_window* h, const lg::WindowArgs& w, cudaStream
     LG_CUDA(cudaLaunchKernelEx(&lc, kern, tq, tk, tv, a));
     return LIGGUF_ATTN_OK;
 }
+// CTAs of the few-rows form that leave partial sums: one wave of two an SM at most.
+long long few_most_items(int sms) { return 2ll * sms; }
+
+template <typename T, typename Out, int D, int kGroups>
+int launch_window_few(const ligguf_window* h, const lg::WindowArgs& w, cudaStream_t st) {
+    constexpr bool bf16 = lg::KvTraits<T>::kBf16;
+    const int device = h->cfg.device;
+    alignas(64) CUtensorMap tk, tv;
+    int rc;
+    if ((rc = make_rows_tmap(&tk, w.k, bf16, D, w.kv_heads, w.k_stride, w.m, w.batch, w.k_batch, lg::kFewKeys)) ||
+        (rc = make_rows_tmap(&tv, w.v, bf16, D, w.kv_heads, w.v_stride, w.m, w.batch, w.v_batch, lg::kFewKeys)))
+        return rc;
+    auto kern = lg::window_few_kernel<T, Out, D, kGroups>;
+    static bool attr_done[64] = {};
+    if (device >= 64 || !attr_done[device]) {
+        LG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lg::FewSmem<D>::kTotal)));
+        if (device < 64) attr_done[device] = true;
+    }
+    lg::WindowFewArgs f = {};
+    f.w = w;
+    f.parts = h->parts;
+    f.err = h->d_err;
+    // Splits: one wave of two CTAs an SM, at least two tiles each.
+    const long long pairs = static_cast<long long>(w.batch) * w.kv_heads;
+    const long long keys = w.window ? std::min<long long>(w.m, static_cast<long long>(w.window) + w.n + w.sinks + 2 * lg::kFewKeys) : w.m;
+    const long long tiles = (keys + lg::kFewKeys - 1) / lg::kFewKeys;
+    f.splits = static_cast<int>(std::max(1ll, std::min(few_most_items(h->num_sms) / pairs, (tiles + 1) / 2)));
+    cudaLaunchConfig_t lc = {};
+    lc.gridDim = dim3(f.splits, w.kv_heads, w.batch);
+    lc.blockDim = dim3(32 * lg::kFewWarps);
+    lc.dynamicSmemBytes = lg::FewSmem<D>::kTotal;
+    lc.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    lc.attrs = attr;
+    lc.numAttrs = 1;
+    LG_CUDA(cudaLaunchKernelEx(&lc, kern, tk, tv, f));
+    if (f.splits == 1) return LIGGUF_ATTN_OK;
+    lc.gridDim = dim3(w.n * (w.q_heads / w.kv_heads), w.kv_heads, w.batch);
+    lc.blockDim = dim3(D);
+    lc.dynamicSmemBytes = 0;
+    LG_CUDA(cudaLaunchKernelEx(&lc, lg::window_join_kernel<Out, D>, f));
+    return LIGGUF_ATTN_OK;
+}
+
+template <typename T, typename Out, int D>
+int launch_window_d(const ligguf_window* h, const lg::WindowArgs& a, cudaStream_t st) {
+    // Few rows a KV head: all of them against each key tile once, the keys split over the SMs.  Up to 64 rows this
+    // is bound by K and V; the tensor-core form reads them once a head and gives a head's keys to one SM.
+    const int rows = a.n * (a.q_heads / a.kv_heads);
+    if (rows <= lg::kFewRows && a.batch <= 65535 && a.kv_heads <= 65535) {
+        if (rows <= 16) return launch_window_few<T, Out, D, 1>(h, a, st);
+        return rows <= 32 ? launch_window_few<T, Out, D, 2>(h, a, st) : launch_window_few<T, Out, D, 4>(h, a, st);
+    }
+    return launch_window_tc<T, Out, D>(h, a, st);
+}
 template <typename T, typename Out>
 int launch_window(const ligguf_window* h, const lg::WindowArgs& a, cudaStream_t st) {
-    return h->cfg.head_dim == 64 ? launch_window_tc<T, Out, 64>(h, a, st) : launch_window_tc<T, Out, 128>(h, a, st);
+    return h->cfg.head_dim == 64 ? launch_window_d<T, Out, 64>(h, a, st) : launch_window_d<T, Out, 128>(h, a, st);
 }
 
 }  // namespace
@@ -728,6 +787,7 @@ int ligguf_cuda_kv4_status(ligguf_kv4* h, void* stream) {
 int ligguf_cuda_window_free(ligguf_window* h) {
     if (!h) return LIGGUF_ATTN_OK;
     DeviceGuard dg(h->cfg.device);
+    cudaFree(h->parts);
     if (h->h_err) cudaFreeHost(h->h_err);
     delete h;
     return LIGGUF_ATTN_OK;
@@ -760,10 +820,17 @@ int ligguf_cuda_window_init(const ligguf_window_cfg* cfg, ligguf_window** out) {
     ligguf_window* h = new (std::nothrow) ligguf_window();
     if (!h) return fail(LIGGUF_ATTN_ENOMEM, "host memory");
     h->cfg = c;
-    if ((rc = make_err_word(&h->h_err, &h->d_err))) {
+    auto bail = [&](int code) {
         ligguf_cuda_window_free(h);
-        return rc;
+        return code;
+    };
+    if (cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, c.device) != cudaSuccess)
+        return bail(fail(LIGGUF_ATTN_ECUDA, "cudaDeviceGetAttribute failed"));
+    if (cudaMalloc(&h->parts, few_most_items(h->num_sms) * lg::kFewRows * (c.head_dim + 2) * sizeof(float)) != cudaSuccess) {
+        (void)cudaGetLastError();
+        return bail(fail(LIGGUF_ATTN_ENOMEM, "handle buffers"));
     }
+    if ((rc = make_err_word(&h->h_err, &h->d_err))) return bail(rc);
     *out = h;
     return LIGGUF_ATTN_OK;
 }
