@@ -17,7 +17,6 @@ import numpy as np
 
 from . import _lib
 from ._lib import Kv4Cfg, QkRopeCfg, RopeCfg, WindowCfg, check
-from .attn import _stream
 
 __all__ = ["RopeConfig", "QkRopeConfig", "QkRope", "Kv4Config", "Kv4Cache", "WindowConfig", "WindowAttention"]
 
@@ -27,6 +26,22 @@ SCALINGS = {"none": _lib.ROPE_SCALE_NONE, "linear": _lib.ROPE_SCALE_LINEAR, "ble
 
 def _p(x):
     return x if x is None or isinstance(x, int) else x.data_ptr()
+
+
+_raw_stream = None
+
+
+def _stream(stream, device):
+    """The stream's handle; by default torch's current stream of the handle's device, asked for without making a
+    Stream object (3 us, more than a small call's whole kernel)."""
+    if stream is not None:
+        return stream if isinstance(stream, int) else stream.cuda_stream
+    global _raw_stream
+    if _raw_stream is None:
+        import torch
+        _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+            (lambda device: torch.cuda.current_stream(device).cuda_stream)
+    return _raw_stream(device)
 
 
 @dataclass
@@ -125,7 +140,7 @@ class QkRope(_Handle):
                   stream=None):
         """n tokens at pos0 + i, or at d_pos[i] (device int32)."""
         rc = self.lib.ligguf_cuda_qk_rope_async(self._h, n, pos0, _p(d_pos), _p(q), _p(k), _p(q_gamma), _p(k_gamma),
-                                                _p(q_out), _p(k_out), _stream(stream))
+                                                _p(q_out), _p(k_out), _stream(stream, self.cfg.device))
         if rc:
             check(rc, "ligguf_cuda_qk_rope_async")
 
@@ -184,7 +199,7 @@ class Kv4Cache(_Handle):
         """A prompt's n tokens into sequence ``seq``; the rotated queries and the rows as the cache holds them
         where an output is given."""
         rc = self.lib.ligguf_cuda_kv4_append_async(self._h, layer, seq, pos0, n, _p(q), _p(k), _p(v), _p(q_out),
-                                                   _p(k_rows), _p(v_rows), _stream(stream))
+                                                   _p(k_rows), _p(v_rows), _stream(stream, self.cfg.device))
         if rc:
             check(rc, "ligguf_cuda_kv4_append_async")
 
@@ -192,28 +207,28 @@ class Kv4Cache(_Handle):
                      stream=None):
         """One token of each of the first n_rows sequences, at ``pos`` or d_pos[r] (device int32, negative: idle)."""
         rc = self.lib.ligguf_cuda_kv4_decode_async(self._h, layer, n_rows, pos, _p(d_pos), _p(q), _p(k), _p(v),
-                                                   _p(out), _p(k_rows), _p(v_rows), _stream(stream))
+                                                   _p(out), _p(k_rows), _p(v_rows), _stream(stream, self.cfg.device))
         if rc:
             check(rc, "ligguf_cuda_kv4_decode_async")
 
     def read_async(self, layer: int, seq: int, pos0: int, n: int, k_rows, v_rows, stream=None):
         """Cached positions as rows of ``rows_type``."""
         check(self.lib.ligguf_cuda_kv4_read_async(self._h, layer, seq, pos0, n, _p(k_rows), _p(v_rows),
-                                                  _stream(stream)), "ligguf_cuda_kv4_read_async")
+                                                  _stream(stream, self.cfg.device)), "ligguf_cuda_kv4_read_async")
 
     def load_async(self, layer: int, seq0: int, n_seqs: int, pos0: int, n: int, k_blocks, v_blocks, stream=None):
         """Q4_0 blocks [n_seqs][n][n_kv_heads*head_dim/32][18 bytes] into the cache, bit for bit."""
         check(self.lib.ligguf_cuda_kv4_load_async(self._h, layer, seq0, n_seqs, pos0, n, _p(k_blocks), _p(v_blocks),
-                                                  _stream(stream)), "ligguf_cuda_kv4_load_async")
+                                                  _stream(stream, self.cfg.device)), "ligguf_cuda_kv4_load_async")
 
     def store_async(self, layer: int, seq0: int, n_seqs: int, pos0: int, n: int, k_blocks, v_blocks, stream=None):
         """The same out of the cache."""
         check(self.lib.ligguf_cuda_kv4_store_async(self._h, layer, seq0, n_seqs, pos0, n, _p(k_blocks), _p(v_blocks),
-                                                   _stream(stream)), "ligguf_cuda_kv4_store_async")
+                                                   _stream(stream, self.cfg.device)), "ligguf_cuda_kv4_store_async")
 
     def status(self, stream=None):
         """Waits for the stream; raises if a decode met a position beyond the context or gave up waiting."""
-        check(self.lib.ligguf_cuda_kv4_status(self._h, _stream(stream)), "ligguf_cuda_kv4_status")
+        check(self.lib.ligguf_cuda_kv4_status(self._h, _stream(stream, self.cfg.device)), "ligguf_cuda_kv4_status")
 
 
 @dataclass
@@ -251,9 +266,9 @@ class WindowAttention(_Handle):
         """n queries a sequence over m rows of keys and values; query i at d_pos0[b] + i (default: the last of the
         sequence's d_lens[b], or m, keys)."""
         rc = self.lib.ligguf_cuda_window_attn_async(self._h, batch, n, m, _p(q), _p(k), _p(v), _p(d_pos0), _p(d_lens),
-                                                    _p(out), _stream(stream))
+                                                    _p(out), _stream(stream, self.cfg.device))
         if rc:
             check(rc, "ligguf_cuda_window_attn_async")
 
     def status(self, stream=None):
-        check(self.lib.ligguf_cuda_window_status(self._h, _stream(stream)), "ligguf_cuda_window_status")
+        check(self.lib.ligguf_cuda_window_status(self._h, _stream(stream, self.cfg.device)), "ligguf_cuda_window_status")
