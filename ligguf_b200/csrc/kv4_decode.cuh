@@ -9,7 +9,7 @@
 // from the packed codes:
 //   - Keys: a code n (0..15) masked into the low mantissa bits of a half is the subnormal n * 2^-24, and
 //     shifted by a nibble n * 2^-20: exact operands that cost one AND for two codes.  The powers of two are
-//     taken out of the fp32 results, and the -8 of (n - 8) d enters as the products' initial value.  The
+//     taken out of the fp32 results, and the -8 of (n - 8) d is added to a group's sum.  The
 //     tensor cores align products by their operands' exponent fields and cut off what lies 24 bits below the
 //     largest, and a subnormal's field is that of 2^-14: so the queries' hi parts are whole numbers, which
 //     makes every product and sum of hi parts exact, cut or not.
@@ -65,23 +65,27 @@ struct Kv4DecodeArgs {
 // Error word of the status call, beside the waits' codes: a decode position beyond the context.
 enum : int { KERR_POSITION = 16 };
 
-constexpr int kKv4Warps = 8;
-constexpr int kKv4Threads = 32 * kKv4Warps;
-constexpr int kKv4MinUnits = 2 * kKv4Warps;  // units a block has at least: fewer blocks share a short context
+// Eight warps a block; two blocks an SM, or one of twice the registers for eight heads a KV head.  (One block of
+// sixteen warps is slower: nothing covers its starts and joins. 24 sequences: 58.8 us against 47.)
+__host__ __device__ constexpr int kv4_warps(int) { return 8; }
+__host__ __device__ constexpr int kv4_blocks_per_sm(int nrep) { return nrep > 4 ? 1 : 2; }
 // Units that an item counts beside its tiles and its token: what a block spends on entering and joining an
 // item, in tiles.
 constexpr int kKv4ItemUnits = 24;
+// Units a block has at least: an item is not cut up for fewer tiles than the join of its parts costs.
+constexpr int kKv4MinUnits = 24;
 
 // Floats of one partial result: o [NREP][D], m [NREP], l [NREP], in whole 16 bytes.
 __host__ __device__ constexpr int kv4_part_floats(int nrep, int dim) { return (nrep * (dim + 2) + 3) / 4 * 4; }
 
 template <int D, int NREP>
 struct Kv4DecodeSmem {
+    static constexpr int kWarps = kv4_warps(NREP);
     static constexpr int kStages = D == 128 ? 2 : 4;  // pairs of tiles a warp has in flight
     static constexpr int kParts = NREP > 4 ? 2 : 1;   // hi and lo queries as columns of one operand, or two operands
     static constexpr int kRow = D + 8;                // floats of a head's row of kO: two heads apart, other banks
     static constexpr size_t kRing = 0;
-    static constexpr size_t kFrag = kRing + size_t(kKv4Warps) * kStages * 2 * Kv4<D>::kTileBytes;  // [kParts][D/16][32] uint2
+    static constexpr size_t kFrag = kRing + size_t(kWarps) * kStages * 2 * Kv4<D>::kTileBytes;  // [kParts][D/16][32] uint2
     static constexpr size_t kSum = kFrag + size_t(kParts) * (D / 16) * 32 * 8;                     // [kParts * 8][D/32]
     static constexpr size_t kScale = kSum + size_t(kParts) * 8 * (D / 32) * 4;                     // [8]
     static constexpr size_t kQ = kScale + 8 * 4;
@@ -90,11 +94,12 @@ struct Kv4DecodeSmem {
     static constexpr size_t kVn = kKn + D * 4;
     static constexpr size_t kCs = kVn + D * 4;
     static constexpr size_t kO = kCs + D / 2 * 8;                             // [warps][NREP][kRow]
-    static constexpr size_t kM = kO + size_t(kKv4Warps) * NREP * kRow * 4;    // [warps + 1][NREP]
-    static constexpr size_t kL = kM + (kKv4Warps + 1) * NREP * 4;
-    static constexpr size_t kJoin = (kL + (kKv4Warps + 1) * NREP * 4 + 15) / 16 * 16;  // sums of a join's groups
-    static constexpr size_t kBar = kJoin + kKv4Threads * 16;
-    static constexpr size_t kMisc = kBar + kKv4Warps * kStages * 8;
+    static constexpr size_t kM = kO + size_t(kWarps) * NREP * kRow * 4;  // [warps + 1][NREP]
+    static constexpr size_t kL = kM + (kWarps + 1) * NREP * 4;
+    static constexpr size_t kF = kL + (kWarps + 1) * NREP * 4;           // [warps + 1][NREP] factors, [NREP] M, [NREP] l
+    static constexpr size_t kJoin = (kF + (kWarps + 3) * NREP * 4 + 15) / 16 * 16;  // sums of a join's groups
+    static constexpr size_t kBar = kJoin + size_t(kWarps) * 32 * 16;
+    static constexpr size_t kMisc = kBar + kWarps * kStages * 8;
     static constexpr size_t kFactors = kMisc + 16;  // [NREP] 1 / sum, then [blocks][NREP]
     static constexpr size_t total(int blocks) { return kFactors + size_t(blocks + 1) * NREP * 4; }
 };
@@ -409,9 +414,8 @@ struct Kv4Warp {
 #pragma unroll
             for (int gr = 0; gr < 2; ++gr) {
                 const int i = ch * 2 + gr;
-                float s[4] = {c[0][i][0], c[0][i][1], c[0][i][0], c[0][i][1]}, s2[4];
-                if constexpr (kWide)  // sums of their own: added to those of the hi parts they would be cut off
-                    s2[0] = s2[2] = c[1][i][0], s2[1] = s2[3] = c[1][i][1];
+                // (lo parts of eight heads in sums of their own: added to those of the hi parts they would be cut off)
+                float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
                     const int j = 2 * i + u;
@@ -420,7 +424,9 @@ struct Kv4Warp {
                     mma_f16(s, a0, a1, a2, a3, b[0][j][0], b[0][j][1], s[0], s[1], s[2], s[3]);
                     if constexpr (kWide) mma_f16(s2, a0, a1, a2, a3, b[1][j][0], b[1][j][1], s2[0], s2[1], s2[2], s2[3]);
                 }
-                if constexpr (kWide) s[0] += s2[0], s[1] += s2[1], s[2] += s2[2], s[3] += s2[3];
+                s[0] += c[0][i][0], s[1] += c[0][i][1], s[2] += c[0][i][0], s[3] += c[0][i][1];
+                if constexpr (kWide)
+                    s[0] += s2[0] + c[1][i][0], s[1] += s2[1] + c[1][i][1], s[2] += s2[2] + c[1][i][0], s[3] += s2[3] + c[1][i][1];
                 x[0] = fmaf(s[0], ks[0][i], x[0]);
                 x[1] = fmaf(s[1], ks[0][i], x[1]);
                 x[2] = fmaf(s[2], ks[1][i], x[2]);
@@ -617,10 +623,11 @@ struct Kv4Warp {
 };
 
 template <typename In, int D, int NREP>
-__global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kernel(const Kv4DecodeArgs a) {
+__global__ void __launch_bounds__(32 * kv4_warps(NREP), kv4_blocks_per_sm(NREP)) kv4_decode_kernel(const Kv4DecodeArgs a) {
     using Sm = Kv4DecodeSmem<D, NREP>;
     constexpr int L = D / 8, TB = Kv4<D>::kTileBytes, PF = kv4_part_floats(NREP, D);
     constexpr unsigned S = Sm::kStages;
+    constexpr int kWarps = Sm::kWarps, kThreads = 32 * kWarps;
     extern __shared__ __align__(128) uint8_t smem[];
     uint2* frag = reinterpret_cast<uint2*>(smem + Sm::kFrag);
     float* sums = reinterpret_cast<float*>(smem + Sm::kSum);
@@ -643,8 +650,8 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
     }
     if (threadIdx.x == 0) *abort = 0;
     if (NREP < 4) {  // columns without a head
-        for (int i = threadIdx.x; i < D / 16 * 32; i += kKv4Threads) frag[i] = make_uint2(0, 0);
-        for (int i = threadIdx.x; i < 8 * (D / 32); i += kKv4Threads) sums[i] = 0.f;
+        for (int i = threadIdx.x; i < D / 16 * 32; i += kThreads) frag[i] = make_uint2(0, 0);
+        for (int i = threadIdx.x; i < 8 * (D / 32); i += kThreads) sums[i] = 0.f;
         if (threadIdx.x < 8) scales[threadIdx.x] = 1.f;
     }
     // The norm weights, which no kernel writes.
@@ -669,9 +676,9 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
             if (pos >= 0 && pos < a.n_context) continue;
             if (pos >= 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = KERR_POSITION;
             const float z[8] = {};
-            for (int u = threadIdx.x; u < a.q_heads * L; u += kKv4Threads)
+            for (int u = threadIdx.x; u < a.q_heads * L; u += kThreads)
                 store8(static_cast<In*>(a.out) + (static_cast<long long>(r) * a.q_heads * L + u) * 8, z);
-            for (int u = threadIdx.x; u < a.kv_heads * L; u += kKv4Threads) {
+            for (int u = threadIdx.x; u < a.kv_heads * L; u += kThreads) {
                 const long long at = (static_cast<long long>(r) * a.kv_heads * L + u) * 8;
                 if (a.k_rows) store_rows8(a.k_rows, a.rows_type, at, z);
                 if (a.v_rows) store_rows8(a.v_rows, a.rows_type, at, z);
@@ -718,6 +725,18 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
     enter(in, u0);
     if (in.t1 <= 0 && in.next > u1) return;  // the share ends before the item's first tile
     Cursor at = in;
+    // The rows of an item that this warp prepares: heads, then (with the item's last unit) the token's key and value.
+    constexpr int kRounds = (NREP + 2 + kWarps - 1) / kWarps;
+    auto load_rows = [&](const Cursor& c, float (&x)[8], int job) {
+        if (job >= NREP + (c.next <= u1 ? 2 : 0)) return;
+        const In* src = job < NREP    ? static_cast<const In*>(a.q) + c.row * a.q_stride + (c.head * NREP + job) * D
+                        : job == NREP ? static_cast<const In*>(a.k) + c.row * a.k_stride + c.head * D
+                                      : static_cast<const In*>(a.v) + c.row * a.v_stride + c.head * D;
+        load8(src + lane % L * 8, x);
+    };
+    float x[8] = {};
+    load_rows(at, x, warp);  // on their way while the copies are requested
+    const double turn = threadIdx.x < a.pairs ? a.turns[threadIdx.x] : 0.0;
     unsigned issued = 0, taken = 0;
     bool more = true;
     auto fill = [&]() {  // requests pairs until the ring is full or the share's end
@@ -735,32 +754,36 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
                 if (two) bulk_copy_g2s(dst + TB, in.tiles + static_cast<long long>(kv4_tile_of(in.r, in.t + 1)) * TB, TB, &bars[s]);
             }
             ++issued;
-            in.t += 2 * kKv4Warps;
+            in.t += 2 * kWarps;
         }
     };
     fill();
 
     Kv4Warp<D, NREP> acc;
     int seg0 = u0;  // first unit of the current item in this share
+    int turned = -1;  // the row whose rotations are in shared memory
+    // Items shared with other blocks: at most the share's first and its last.  They are joined at the end, when the
+    // tickets have long come back.
+    struct Shared {
+        long long item;
+        int first, parts, lead, ticket;  // blocks that have parts, the slot of the first block's
+    } lead_item = {0, 0, 0, 0, -1}, last_item = {0, 0, 0, 0, -1};
     for (int seg = 0;; ++seg) {
         const int pos = at.r.pos, g = at.head;
         const int item0 = at.next - at.units + kKv4ItemUnits;  // the item's first tile
         const bool own = at.next <= u1;  // the item's last unit, the token itself, is in this share
         const long long item = static_cast<long long>(at.row) * a.kv_heads + g;
         // Queries (and the token's own key and value) of the item.
-        for (int job = warp, round = 0; round < (NREP + 2 + kKv4Warps - 1) / kKv4Warps; job += kKv4Warps, ++round) {
+        if (at.row != turned) {  // (a row's heads follow one another)
+            if (threadIdx.x < a.pairs) cs[threadIdx.x] = rope_turn(turn, pos, a.magnitude);
+            turned = at.row;
+            __syncthreads();
+        }
+#pragma unroll
+        for (int round = 0; round < kRounds; ++round) {
+            const int job = warp + round * kWarps;
             const bool on = job < NREP + (own ? 2 : 0), isq = job < NREP, isk = job == NREP;
-            float x[8];
-            if (on) {
-                const In* src = isq   ? static_cast<const In*>(a.q) + at.row * a.q_stride + (g * NREP + job) * D
-                                : isk ? static_cast<const In*>(a.k) + at.row * a.k_stride + g * D
-                                      : static_cast<const In*>(a.v) + at.row * a.v_stride + g * D;
-                load8(src + lane % L * 8, x);
-            }
-            if (round == 0) {  // with the loads in flight
-                if (threadIdx.x < a.pairs) cs[threadIdx.x] = rope_turn(a.turns[threadIdx.x], pos, a.magnitude);
-                __syncthreads();
-            }
+            if (round) load_rows(at, x, job);
             if (!on) continue;
             float* dst = isq ? qs + job * D : isk ? kn : vn;
             const bool rot = isq || isk;
@@ -790,14 +813,12 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
         }
         __syncthreads();
         acc.start(frag, sums, scales, lane);
-        for (; at.t < at.t1; at.t += 2 * kKv4Warps) {
+        for (; at.t < at.t1; at.t += 2 * kWarps) {
             const unsigned s = taken % S;
-            if (!__all_sync(0xffffffffu, mbar_wait_bounded(&bars[s], (taken / S) & 1, deadline, abort))) {
-                if (lane == 0) {
-                    *abort = 1;
-                    *reinterpret_cast<volatile int*>(a.err) = KERR_TIMEOUT_FULL;
-                }
-                break;
+            if (!mbar_wait_bounded(&bars[s], (taken / S) & 1, deadline, abort)) {
+                // (the tile is worked on as it is; the block stops at the next barrier)
+                *abort = 1;
+                *reinterpret_cast<volatile int*>(a.err) = KERR_TIMEOUT_FULL;
             }
             acc.pair(ring + s * 2 * TB, at.r, kv4_tile_of(at.r, at.t) * kKv4Tile,
                      at.t + 1 < at.t1 ? kv4_tile_of(at.r, at.t + 1) * kKv4Tile : -1, lane);
@@ -805,110 +826,131 @@ __global__ void __launch_bounds__(kKv4Threads, NREP > 4 ? 1 : 2) kv4_decode_kern
             ++taken;
             fill();
         }
+        const int next = at.next, begin = at.next - at.units;
+        const bool more_items = advance(at);
+        if (more_items) load_rows(at, x, warp);  // of the next item, while this one is joined
         acc.finish(so + warp * NREP * Sm::kRow, sm + warp * NREP, sl + warp * NREP, lane);
         if (own)  // the token itself: one key whose weight is 1 relative to its own score
-            for (int h = warp; h < NREP; h += kKv4Warps) {
-                float x = 0.f;
+            for (int h = warp; h < NREP; h += kWarps) {
+                float y = 0.f;
 #pragma unroll
-                for (int i = 0; i < D / 32; ++i) x = fmaf(qs[h * D + lane + 32 * i], kn[lane + 32 * i], x);
-                x = warp_sum(x);
-                if (lane == 0) sm[kKv4Warps * NREP + h] = x, sl[kKv4Warps * NREP + h] = 1.f;
+                for (int i = 0; i < D / 32; ++i) y = fmaf(qs[h * D + lane + 32 * i], kn[lane + 32 * i], y);
+                y = warp_sum(y);
+                if (lane == 0) sm[kWarps * NREP + h] = y, sl[kWarps * NREP + h] = 1.f;
             }
         __syncthreads();
         if (*abort) break;  // raised before the barrier: every thread sees it
-        // Join the warps.
+        // Join the warps: their factors, a head a warp, then the sums.
+        float* fac = reinterpret_cast<float*>(smem + Sm::kF);
+        for (int h = warp; h < NREP; h += kWarps) {
+            const bool on = lane < kWarps + (own ? 1 : 0);
+            const float m = on ? sm[lane * NREP + h] : -1e30f;
+            const float M = warp_max(m), f = ex2(m - M);
+            const float l = warp_sum(on ? sl[lane * NREP + h] * f : 0.f);
+            if (on) fac[lane * NREP + h] = f;
+            if (lane == 0) fac[(kWarps + 1) * NREP + h] = M, fac[(kWarps + 2) * NREP + h] = l;
+        }
+        __syncthreads();
         const bool whole = own && seg0 <= item0;  // no other block has a part of this item
         In* out = static_cast<In*>(a.out) + item * NREP * D;
         float* mine = a.parts + (static_cast<long long>(bx) * 2 + (seg ? 1 : 0)) * PF;
-        for (int i = threadIdx.x; i < NREP * D; i += kKv4Threads) {
+        for (int i = threadIdx.x; i < NREP * D; i += kThreads) {
             const int h = i / D, d = i % D;
-            float M = own ? sm[kKv4Warps * NREP + h] : -1e30f, mw[kKv4Warps];
+            float osum = own ? fac[kWarps * NREP + h] * vn[d] : 0.f;
 #pragma unroll
-            for (int w = 0; w < kKv4Warps; ++w) mw[w] = sm[w * NREP + h], M = fmaxf(M, mw[w]);
-            const float f0 = own ? ex2(sm[kKv4Warps * NREP + h] - M) : 0.f;
-            float lsum = f0, osum = own ? f0 * vn[d] : 0.f;
-#pragma unroll
-            for (int w = 0; w < kKv4Warps; ++w) {
-                const float f = ex2(mw[w] - M);
-                lsum = fmaf(sl[w * NREP + h], f, lsum);
-                osum = fmaf(so[(w * NREP + h) * Sm::kRow + d], f, osum);
-            }
+            for (int w = 0; w < kWarps; ++w) osum = fmaf(so[(w * NREP + h) * Sm::kRow + d], fac[w * NREP + h], osum);
+            const float M = fac[(kWarps + 1) * NREP + h], l = fac[(kWarps + 2) * NREP + h];
             if (whole) {
-                out[i] = KvTraits<In>::from_float(osum / lsum);
+                out[i] = KvTraits<In>::from_float(osum / l);
             } else {
                 mine[i] = osum;
-                if (d == 0) mine[NREP * D + h] = M, mine[NREP * D + NREP + h] = lsum;
+                if (d == 0) mine[NREP * D + h] = M, mine[NREP * D + NREP + h] = l;
             }
         }
+        __syncthreads();
         if (!whole) {
-            // Blocks b0..b1 have parts of the item: those whose shares meet [item0, at.next).
-            const int b0 = item0 / share, b1 = (at.next - 1) / share, n = b1 - b0 + 1;
-            __syncthreads();
-            if (threadIdx.x == 0) {
+            // Blocks b0..b1 have parts of the item: those whose shares meet [item0, next).  Block b0's lies in its
+            // second slot when the item is not the first of its share.
+            const int b0 = item0 / share, b1 = (next - 1) / share;
+            Shared e = {item, b0, b1 - b0 + 1, b0 * share < begin ? 1 : 0, -1};
+            if (threadIdx.x == 0)
                 // The block's part, ordered before this by the barrier, is out before the ticket; what the
                 // other blocks put out before theirs is seen after it.
-                int done;
-                asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(done) : "l"(a.tickets + item) : "memory");
-                *last = done == n - 1;
-                if (done == n - 1) a.tickets[item] = 0;
+                asm volatile("atom.acq_rel.gpu.global.add.s32 %0, [%1], 1;" : "=r"(e.ticket) : "l"(a.tickets + item) : "memory");
+            if (seg)
+                last_item = e;
+            else
+                lead_item = e;
+        }
+        seg0 = next;
+        if (!more_items) break;
+    }
+    // Joins the parts of an item that other blocks share, in the last of them to be done.
+    auto join = [&](const Shared& e) {
+        if (e.parts == 0) return;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            *last = e.ticket == e.parts - 1;
+            if (*last) a.tickets[e.item] = 0;
+        }
+        __syncthreads();
+        if (!*last) return;
+        const float* parts = a.parts + static_cast<long long>(e.first) * 2 * PF;
+        auto part = [&](int w) { return parts + (w ? w * 2 : e.lead) * PF; };
+        // Threads in groups, one 16-byte column a thread; a group takes every kGroups-th part.
+        constexpr int kCols = NREP * D / 4, kGroups = kThreads / kCols, kAhead = 8;
+        const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
+        float4 y8[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u)
+            if (grp + u * kGroups < e.parts) y8[u] = __ldcg(reinterpret_cast<const float4*>(part(grp + u * kGroups)) + col);
+        float* inv = reinterpret_cast<float*>(smem + Sm::kFactors);
+        float* fac = inv + NREP;
+        for (int h = warp; h < NREP; h += kWarps) {  // the parts' factors, a head a warp
+            float m0 = -1e30f, l0 = 0.f;  // of part `lane`, which is all of them up to 32
+            if (lane < e.parts) m0 = __ldcg(part(lane) + NREP * D + h), l0 = __ldcg(part(lane) + NREP * D + NREP + h);
+            float M = m0;
+            for (int w = lane + 32; w < e.parts; w += 32) M = fmaxf(M, __ldcg(part(w) + NREP * D + h));
+            M = warp_max(M);
+            float l = l0 * ex2(m0 - M);
+            if (lane < e.parts) fac[lane * NREP + h] = ex2(m0 - M);
+            for (int w = lane + 32; w < e.parts; w += 32) {
+                const float f = ex2(__ldcg(part(w) + NREP * D + h) - M);
+                fac[w * NREP + h] = f;
+                l = fmaf(__ldcg(part(w) + NREP * D + NREP + h), f, l);
             }
-            __syncthreads();
-            if (*last) {
-                // Block b0's part lies in its second slot when the item is not the first of its share.
-                const int lead = b0 * share < at.next - at.units ? 1 : 0;
-                const float* parts = a.parts + static_cast<long long>(b0) * 2 * PF;
-                auto part = [&](int w) { return parts + (w ? w * 2 : lead) * PF; };
-                // Threads in groups, one 16-byte column a thread; a group takes every kGroups-th part.
-                constexpr int kCols = NREP * D / 4, kGroups = kKv4Threads / kCols, kAhead = 8;
-                const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
-                float4 x[kAhead];
+            l = warp_sum(l);
+            if (lane == 0) inv[h] = 1.f / l;
+        }
+        __syncthreads();
+        float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+        const int h = col * 4 / D;
+        for (int w0 = grp; w0 < e.parts; w0 += kGroups * kAhead) {
 #pragma unroll
-                for (int u = 0; u < kAhead; ++u)
-                    if (grp + u * kGroups < n) x[u] = __ldcg(reinterpret_cast<const float4*>(part(grp + u * kGroups)) + col);
-                float* inv = reinterpret_cast<float*>(smem + Sm::kFactors);
-                float* fac = inv + NREP;
-                if (warp < NREP) {  // the parts' factors, a head a warp
-                    float M = -1e30f, ls = 0.f;
-                    for (int w = lane; w < n; w += 32) M = fmaxf(M, __ldcg(part(w) + NREP * D + warp));
-                    M = warp_max(M);
-                    for (int w = lane; w < n; w += 32) {
-                        const float f = ex2(__ldcg(part(w) + NREP * D + warp) - M);
-                        fac[w * NREP + warp] = f;
-                        ls = fmaf(__ldcg(part(w) + NREP * D + NREP + warp), f, ls);
-                    }
-                    ls = warp_sum(ls);
-                    if (lane == 0) inv[warp] = 1.f / ls;
-                }
-                __syncthreads();
-                float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-                const int h = col * 4 / D;
-                for (int w0 = grp; w0 < n; w0 += kGroups * kAhead) {
-#pragma unroll
-                    for (int u = 0; u < kAhead; ++u) {
-                        const int w = w0 + u * kGroups;
-                        if (w >= n) continue;
-                        const float f = fac[w * NREP + h];
-                        const float4 z = w0 == grp ? x[u] : __ldcg(reinterpret_cast<const float4*>(part(w)) + col);
-                        y.x = fmaf(z.x, f, y.x), y.y = fmaf(z.y, f, y.y), y.z = fmaf(z.z, f, y.z), y.w = fmaf(z.w, f, y.w);
-                    }
-                }
-                float4* join = reinterpret_cast<float4*>(smem + Sm::kJoin);
-                join[threadIdx.x] = y;
-                __syncthreads();
-                if (grp == 0) {
-#pragma unroll
-                    for (int i = 1; i < kGroups; ++i) {
-                        const float4 z = join[i * kCols + col];
-                        y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
-                    }
-                    const float f = inv[h];
-                    store4(out + col * 4, make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
-                }
+            for (int u = 0; u < kAhead; ++u) {
+                const int w = w0 + u * kGroups;
+                if (w >= e.parts) continue;
+                const float f = fac[w * NREP + h];
+                const float4 z = w0 == grp ? y8[u] : __ldcg(reinterpret_cast<const float4*>(part(w)) + col);
+                y.x = fmaf(z.x, f, y.x), y.y = fmaf(z.y, f, y.y), y.z = fmaf(z.z, f, y.z), y.w = fmaf(z.w, f, y.w);
             }
         }
-        seg0 = at.next;
-        if (!advance(at)) break;
-        __syncthreads();  // the next item overwrites what this one's join read
+        float4* sums4 = reinterpret_cast<float4*>(smem + Sm::kJoin);
+        sums4[threadIdx.x] = y;
+        __syncthreads();
+        if (grp == 0) {
+#pragma unroll
+            for (int i = 1; i < kGroups; ++i) {
+                const float4 z = sums4[i * kCols + col];
+                y.x += z.x, y.y += z.y, y.z += z.z, y.w += z.w;
+            }
+            const float f = inv[h];
+            store4(static_cast<In*>(a.out) + e.item * NREP * D + col * 4, make_float4(y.x * f, y.y * f, y.z * f, y.w * f));
+        }
+    };
+    if (!*abort) {  // (the same for every thread: raised before a barrier that all have passed)
+        join(lead_item);
+        join(last_item);
     }
     // After a wait that gave up, the copies in flight land before the block ends.
     for (; taken < issued; ++taken)

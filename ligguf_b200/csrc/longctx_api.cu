@@ -182,9 +182,6 @@ int launch_rope_rows_any(lg::RopeRowsArgs& a, const ligguf_rope_cfg& r, int in_t
     }
 }
 
-// Blocks of the decode kernel resident per SM (its __launch_bounds__ minimum).
-int kv4_blocks_per_sm(int nrep) { return nrep > 4 ? 1 : 2; }
-
 int make_err_word(int** h_err, int** d_err) {
     if (cudaHostAlloc(reinterpret_cast<void**>(h_err), 64, cudaHostAllocMapped) != cudaSuccess)
         return fail(LIGGUF_ATTN_ENOMEM, "mapped error word");
@@ -245,17 +242,17 @@ int launch_kv4_decode(const ligguf_kv4* h, lg::Kv4DecodeArgs& a, cudaStream_t st
     static bool attr_done[64] = {};
     const int device = h->cfg.device;
     if (device >= 64 || !attr_done[device]) {
-        LG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Sm::total(h->num_sms * kv4_blocks_per_sm(NREP)))));
+        LG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Sm::total(h->num_sms * lg::kv4_blocks_per_sm(NREP)))));
         if (device < 64) attr_done[device] = true;
     }
     // As many blocks as fit at once, fewer when the longest visible contexts do not fill them.
     const long long keys = std::min<long long>(h->cfg.n_context, a.window ? 2ll * lg::kKv4Tile + a.window + a.sinks : INT32_MAX);
     const long long units = (keys / lg::kKv4Tile + 2 + lg::kKv4ItemUnits) * a.kv_heads * a.n_rows;
-    const int slots = h->num_sms * kv4_blocks_per_sm(NREP);
+    const int slots = h->num_sms * lg::kv4_blocks_per_sm(NREP);
     cudaLaunchConfig_t lc = {};
     lc.gridDim = dim3(static_cast<unsigned>(std::min<long long>(slots, std::max<long long>(1, units / lg::kKv4MinUnits))));
     a.per_block = 1.0f / static_cast<float>(lc.gridDim.x);
-    lc.blockDim = dim3(lg::kKv4Threads);
+    lc.blockDim = dim3(32 * Sm::kWarps);
     lc.dynamicSmemBytes = Sm::total(slots);
     lc.stream = st;
     cudaLaunchAttribute attr[1];
@@ -606,7 +603,7 @@ int ligguf_cuda_kv4_init(const ligguf_kv4_cfg* cfg, ligguf_kv4** out) {
     }
     if (cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, c.device) != cudaSuccess)
         return bail(fail(LIGGUF_ATTN_ECUDA, "cudaDeviceGetAttribute failed"));
-    const size_t part_bytes = size_t(h->num_sms) * kv4_blocks_per_sm(nrep) * 2 * lg::kv4_part_floats(nrep, D) * sizeof(float);
+    const size_t part_bytes = size_t(h->num_sms) * lg::kv4_blocks_per_sm(nrep) * 2 * lg::kv4_part_floats(nrep, D) * sizeof(float);
     const size_t ticket_bytes = size_t(c.n_seqs) * c.n_kv_heads * sizeof(int);
     if (cudaMalloc(&h->gammas, gbytes) != cudaSuccess || cudaMalloc(&h->parts, part_bytes) != cudaSuccess ||
         cudaMalloc(&h->tickets, ticket_bytes) != cudaSuccess) {
