@@ -86,7 +86,7 @@ struct Kv4DecodeSmem {
     static constexpr int kRow = D + 8;                // floats of a head's row of kO: two heads apart, other banks
     static constexpr size_t kRing = 0;
     static constexpr size_t kFrag = kRing + size_t(kWarps) * kStages * 2 * Kv4<D>::kTileBytes;  // [kParts][D/16][32] uint2
-    static constexpr size_t kSum = kFrag + size_t(kParts) * (D / 16) * 32 * 8;                     // [kParts * 8][D/32]
+    static constexpr size_t kSum = kFrag + size_t(kParts) * (D / 16) * 32 * 8;                     // [kParts][D/32][8]
     static constexpr size_t kScale = kSum + size_t(kParts) * 8 * (D / 32) * 4;                     // [8]
     static constexpr size_t kQ = kScale + 8 * 4;
     static constexpr size_t kGamma = kQ + NREP * D * 4;  // norm weights of q and k
@@ -333,8 +333,8 @@ __device__ __forceinline__ void kv4_query_operands(const float (&x)[8], int head
     }
     constexpr float k8 = -8.f / 16777216.f;
     if (lane < L && (l & 3) == 0) {
-        sums[head * G + (l >> 2)] = k8 * sh;
-        sums[((kWide ? 8 : 4) + head) * G + (l >> 2)] = k8 * sl;
+        sums[(l >> 2) * 8 + head] = k8 * sh;
+        sums[(kWide ? 8 * G : 4) + (l >> 2) * 8 + head] = k8 * sl;
     }
     if (lane == 0) {
         const float down = __int_as_float((127 + e + 14) << 23);  // 2^(e - 10) * 2^24
@@ -372,29 +372,19 @@ template <int D, int NREP>
 struct Kv4Warp {
     static constexpr bool kWide = NREP > 4;  // hi and lo parts as two products
     static constexpr int KS = D / 16, G = D / 32;
-    uint32_t b[kWide ? 2 : 1][KS][2];  // queries, as B operands
-    float c[kWide ? 2 : 1][G][2];      // -8 * sum of a group's queries, of this lane's columns
-    float sx[2];                       // scales of the scores of this lane's two heads
+    // Queries as B operands, and -8 times the sums of their groups, stay in shared memory: two loads a pair of tiles
+    // and k-step cost less than the registers.
+    const uint2* b;   // this lane's, of k-step 0
+    const float2* c;  // this lane's two columns, of group 0
+    float sx[2];      // scales of the scores of this lane's two heads
     float m[2], l[2];                  // running maxima and sums of weights
     float o[KS][4];
 
     // From what kv4_query_operands left in shared memory.
     __device__ __forceinline__ void start(const uint2* frag, const float* sums, const float* scales, int lane) {
         const int t = lane & 3;
-#pragma unroll
-        for (int p = 0; p < (kWide ? 2 : 1); ++p)
-#pragma unroll
-            for (int j = 0; j < KS; ++j) {
-                const uint2 f = frag[(p * KS + j) * 32 + lane];
-                b[p][j][0] = f.x, b[p][j][1] = f.y;
-            }
-#pragma unroll
-        for (int p = 0; p < (kWide ? 2 : 1); ++p)
-#pragma unroll
-            for (int i = 0; i < G; ++i) {
-                c[p][i][0] = sums[(8 * p + 2 * t) * G + i];
-                c[p][i][1] = sums[(8 * p + 2 * t + 1) * G + i];
-            }
+        b = frag + lane;
+        c = reinterpret_cast<const float2*>(sums) + t;
         sx[0] = scales[2 * t], sx[1] = scales[2 * t + 1];
 #pragma unroll
         for (int i = 0; i < 2; ++i) m[i] = -1e30f, l[i] = 0.f;
@@ -402,35 +392,48 @@ struct Kv4Warp {
         for (int i = 0; i < KS; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
     }
 
-    // Raw scores of a tile's positions g (x[0], x[1]) and g + 8 (x[2], x[3]) with this lane's columns.
-    __device__ __forceinline__ void scores(const uint8_t* tp, int lane, float (&x)[4]) const {
-        float ks[2][G];
-        load_scales(tp + Kv4<D>::kKeyScales, lane >> 2, ks);
-        x[0] = x[1] = x[2] = x[3] = 0.f;
+    // Raw scores of kTiles tiles' positions g (x[0], x[1]) and g + 8 (x[2], x[3]) with this lane's columns.
+    template <int kTiles>
+    __device__ __forceinline__ void scores(const uint8_t* tp, int lane, float (&x)[kTiles][4]) const {
+        constexpr int TB = Kv4<D>::kTileBytes;
+#pragma unroll
+        for (int n = 0; n < kTiles; ++n) x[n][0] = x[n][1] = x[n][2] = x[n][3] = 0.f;
 #pragma unroll
         for (int ch = 0; ch < D / 64; ++ch) {
-            const uint4 w4 = lds128(tp + ch * 512 + lane * 16);
-            const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+            uint4 w4[kTiles];
+#pragma unroll
+            for (int n = 0; n < kTiles; ++n) w4[n] = lds128(tp + n * TB + ch * 512 + lane * 16);
 #pragma unroll
             for (int gr = 0; gr < 2; ++gr) {
                 const int i = ch * 2 + gr;
                 // (lo parts of eight heads in sums of their own: added to those of the hi parts they would be cut off)
-                float s[4] = {0.f, 0.f, 0.f, 0.f}, s2[4] = {0.f, 0.f, 0.f, 0.f};
+                float s[kTiles][4] = {}, s2[kTiles][4] = {};
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const int j = 2 * i + u;
-                    const uint32_t lo = w[2 * gr + u], hi = lo >> 8;
-                    const uint32_t a0 = lo & 0x000F000Fu, a2 = lo & 0x00F000F0u, a1 = hi & 0x000F000Fu, a3 = hi & 0x00F000F0u;
-                    mma_f16(s, a0, a1, a2, a3, b[0][j][0], b[0][j][1], s[0], s[1], s[2], s[3]);
-                    if constexpr (kWide) mma_f16(s2, a0, a1, a2, a3, b[1][j][0], b[1][j][1], s2[0], s2[1], s2[2], s2[3]);
+                    const uint2 q = b[(2 * i + u) * 32], r = kWide ? b[(KS + 2 * i + u) * 32] : make_uint2(0, 0);
+#pragma unroll
+                    for (int n = 0; n < kTiles; ++n) {
+                        const uint32_t lo = gr ? (u ? w4[n].w : w4[n].z) : (u ? w4[n].y : w4[n].x), hi = lo >> 8;
+                        const uint32_t a0 = lo & 0x000F000Fu, a2 = lo & 0x00F000F0u, a1 = hi & 0x000F000Fu, a3 = hi & 0x00F000F0u;
+                        mma_f16(s[n], a0, a1, a2, a3, q.x, q.y, s[n][0], s[n][1], s[n][2], s[n][3]);
+                        if constexpr (kWide) mma_f16(s2[n], a0, a1, a2, a3, r.x, r.y, s2[n][0], s2[n][1], s2[n][2], s2[n][3]);
+                    }
                 }
-                s[0] += c[0][i][0], s[1] += c[0][i][1], s[2] += c[0][i][0], s[3] += c[0][i][1];
-                if constexpr (kWide)
-                    s[0] += s2[0] + c[1][i][0], s[1] += s2[1] + c[1][i][1], s[2] += s2[2] + c[1][i][0], s[3] += s2[3] + c[1][i][1];
-                x[0] = fmaf(s[0], ks[0][i], x[0]);
-                x[1] = fmaf(s[1], ks[0][i], x[1]);
-                x[2] = fmaf(s[2], ks[1][i], x[2]);
-                x[3] = fmaf(s[3], ks[1][i], x[3]);
+                const float2 c0 = c[4 * i];
+                float2 c1 = make_float2(0.f, 0.f);
+                if constexpr (kWide) c1 = c[4 * (G + i)];
+#pragma unroll
+                for (int n = 0; n < kTiles; ++n) {
+                    const __half* ks = reinterpret_cast<const __half*>(tp + n * TB + Kv4<D>::kKeyScales) + (lane >> 2) * G + i;
+                    const float k0 = __half2float(ks[0]), k1 = __half2float(ks[8 * G]);
+                    float* y = s[n];
+                    if constexpr (kWide)
+                        y[0] += s2[n][0] + c1.x, y[1] += s2[n][1] + c1.y, y[2] += s2[n][2] + c1.x, y[3] += s2[n][3] + c1.y;
+                    x[n][0] = fmaf(y[0] + c0.x, k0, x[n][0]);
+                    x[n][1] = fmaf(y[1] + c0.y, k0, x[n][1]);
+                    x[n][2] = fmaf(y[2] + c0.x, k1, x[n][2]);
+                    x[n][3] = fmaf(y[3] + c0.y, k1, x[n][3]);
+                }
             }
         }
     }
@@ -475,9 +478,9 @@ struct Kv4Warp {
 #pragma unroll 1
             for (int n = 0; n < 2; ++n, tp += TB, k0 = k1) {
                 if (k0 < 0) return;
-                float x[4], p[4], vs[2][G];
-                scores(tp, lane, x);
-                weights(tp, r, k0, edge(r, k0), true, lane, x, p, vs);
+                float x[1][4], p[4], vs[2][G];
+                scores<1>(tp, lane, x);
+                weights(tp, r, k0, edge(r, k0), true, lane, x[0], p, vs);
 #pragma unroll
                 for (int ch = 0; ch < D / 64; ++ch) {
                     const uint4 w4 = lds128(tp + Kv4<D>::kCodes + ch * 512 + lane * 16);
@@ -500,12 +503,11 @@ struct Kv4Warp {
             const bool second = lane & 2;  // lanes of the lo columns take the second tile
             float x[4], p[4], vs[2][G];
             {
-                float xa[4], xb[4];
-                scores(tp, lane, xa);
-                scores(tp + TB, lane, xb);
+                float xs[2][4];
+                scores<2>(tp, lane, xs);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    x[i] = (second ? xb[i] : xa[i]) + __shfl_xor_sync(0xffffffffu, second ? xa[i] : xb[i], 2);
+                    x[i] = (second ? xs[1][i] : xs[0][i]) + __shfl_xor_sync(0xffffffffu, second ? xs[0][i] : xs[1][i], 2);
             }
             weights(second ? tp + TB : tp, r, second ? k1 : k0, k1 < 0 || edge(r, k0) || edge(r, k1), !second || k1 >= 0, lane,
                     x, p, vs);
@@ -559,19 +561,6 @@ struct Kv4Warp {
         for (int j = 0; j < KS; ++j) o[j][0] *= f0, o[j][1] *= f1, o[j][2] *= f0, o[j][3] *= f1;
     }
 
-    __device__ __forceinline__ static void load_scales(const uint8_t* s, int g, float (&out)[2][G]) {
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            if constexpr (G == 4) {
-                const uint2 u = lds64(s + (g + 8 * r) * 8);
-                const float2 x = unpack_f16(u.x), y = unpack_f16(u.y);
-                out[r][0] = x.x, out[r][1] = x.y, out[r][2] = y.x, out[r][3] = y.y;
-            } else {
-                const float2 x = unpack_f16(*reinterpret_cast<const uint32_t*>(s + (g + 8 * r) * 4));
-                out[r][0] = x.x, out[r][1] = x.y;
-            }
-        }
-    }
     // The value scales, and for both rows an exponent E with |scale| < 2^E for every group.
     __device__ __forceinline__ static float2 load_value_scales(const uint8_t* s, int g, float (&out)[2][G]) {
         float e[2];
