@@ -509,8 +509,10 @@ struct Kv4Warp {
                 for (int i = 0; i < 4; ++i)
                     x[i] = (second ? xs[1][i] : xs[0][i]) + __shfl_xor_sync(0xffffffffu, second ? xs[0][i] : xs[1][i], 2);
             }
-            weights(second ? tp + TB : tp, r, second ? k1 : k0, k1 < 0 || edge(r, k0) || edge(r, k1), !second || k1 >= 0, lane,
-                    x, p, vs);
+            // (k1 > k0, so these two are the first's lower and the second's upper edge; a tile of first tokens, below the
+            // window, counts as an edge)
+            const bool masked = k1 < 0 || k0 < r.first || k1 + kKv4Tile > r.pos;
+            weights(second ? tp + TB : tp, r, second ? k1 : k0, masked, !second || k1 >= 0, lane, x, p, vs);
 #pragma unroll
             for (int ch = 0; ch < D / 64; ++ch) {
                 const uint4 wa4 = lds128(tp + Kv4<D>::kCodes + ch * 512 + lane * 16);
@@ -728,25 +730,30 @@ __global__ void __launch_bounds__(32 * kv4_warps(NREP), kv4_blocks_per_sm(NREP))
     const double turn = threadIdx.x < a.pairs ? a.turns[threadIdx.x] : 0.0;
     unsigned issued = 0, taken = 0;
     bool more = true;
-    auto fill = [&]() {  // requests pairs until the ring is full or the share's end
-        while (more && issued < taken + S) {
-            if (in.t >= in.t1) {
-                more = advance(in);
-                continue;
-            }
-            if (lane == 0) {
-                const unsigned s = issued % S;
-                uint8_t* dst = ring + s * 2 * TB;
-                const bool two = in.t + 1 < in.t1;
-                mbar_arrive_expect_tx(&bars[s], two ? 2 * TB : TB);
-                bulk_copy_g2s(dst, in.tiles + static_cast<long long>(kv4_tile_of(in.r, in.t)) * TB, TB, &bars[s]);
-                if (two) bulk_copy_g2s(dst + TB, in.tiles + static_cast<long long>(kv4_tile_of(in.r, in.t + 1)) * TB, TB, &bars[s]);
-            }
-            ++issued;
-            in.t += 2 * kWarps;
+    auto request = [&]() {  // the next pair of this warp, if there is one
+        while (in.t >= in.t1) {
+            more = more && advance(in);
+            if (!more) return;
         }
+        if (lane == 0) {
+            const unsigned s = issued % S;
+            uint8_t* dst = ring + s * 2 * TB;
+            const int first = kv4_tile_of(in.r, in.t);
+            const uint8_t* src = in.tiles + static_cast<long long>(first) * TB;
+            const int bytes = in.t + 1 < in.t1 ? 2 * TB : TB;
+            mbar_arrive_expect_tx(&bars[s], bytes);
+            if (in.t + 1 != in.r.ns || bytes == TB) {  // neighbours
+                bulk_copy_g2s(dst, src, bytes, &bars[s]);
+            } else {
+                bulk_copy_g2s(dst, src, TB, &bars[s]);
+                bulk_copy_g2s(dst + TB, in.tiles + static_cast<long long>(in.r.tw) * TB, TB, &bars[s]);
+            }
+        }
+        ++issued;
+        in.t += 2 * kWarps;
     };
-    fill();
+#pragma unroll 1
+    for (unsigned s = 0; s < S; ++s) request();
 
     Kv4Warp<D, NREP> acc;
     int seg0 = u0;  // first unit of the current item in this share
@@ -804,16 +811,17 @@ __global__ void __launch_bounds__(32 * kv4_warps(NREP), kv4_blocks_per_sm(NREP))
         acc.start(frag, sums, scales, lane);
         for (; at.t < at.t1; at.t += 2 * kWarps) {
             const unsigned s = taken % S;
-            if (!mbar_wait_bounded(&bars[s], (taken / S) & 1, deadline, abort)) {
+            if (!mbar_try_wait(&bars[s], (taken / S) & 1) && !mbar_wait_bounded(&bars[s], (taken / S) & 1, deadline, abort)) {
                 // (the tile is worked on as it is; the block stops at the next barrier)
                 *abort = 1;
                 *reinterpret_cast<volatile int*>(a.err) = KERR_TIMEOUT_FULL;
             }
-            acc.pair(ring + s * 2 * TB, at.r, kv4_tile_of(at.r, at.t) * kKv4Tile,
-                     at.t + 1 < at.t1 ? kv4_tile_of(at.r, at.t + 1) * kKv4Tile : -1, lane);
+            const int k0 = kv4_tile_of(at.r, at.t) * kKv4Tile;
+            const int k1 = at.t + 1 == at.r.ns ? at.r.tw * kKv4Tile : k0 + kKv4Tile;
+            acc.pair(ring + s * 2 * TB, at.r, k0, at.t + 1 < at.t1 ? k1 : -1, lane);
             __syncwarp();
             ++taken;
-            fill();
+            request();
         }
         const int next = at.next, begin = at.next - at.units;
         const bool more_items = advance(at);
