@@ -73,7 +73,7 @@ __host__ __device__ constexpr int kv4_blocks_per_sm(int nrep) { return nrep > 4 
 // item, in tiles.
 constexpr int kKv4ItemUnits = 24;
 // Units a block has at least: an item is not cut up for fewer tiles than the join of its parts costs.
-constexpr int kKv4MinUnits = 24;
+constexpr int kKv4MinUnits = 16;
 
 // Floats of one partial result: o [NREP][D], m [NREP], l [NREP], in whole 16 bytes.
 __host__ __device__ constexpr int kv4_part_floats(int nrep, int dim) { return (nrep * (dim + 2) + 3) / 4 * 4; }

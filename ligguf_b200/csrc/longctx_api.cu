@@ -102,64 +102,37 @@ int rope_layout(const ligguf_rope_cfg& r) {
     return r.rope_dim % 16 == 0 ? lg::kRopeHalves : lg::kRopeHalvesOdd;
 }
 
-template <typename In, typename Out, int D, int kLayout>
-int launch_rope_units(lg::RopeRowsArgs& a, cudaStream_t st) {
-    // A unit a thread.  Few tokens: 128 a block, a token's heads over several blocks (each computes the rotation
-    // again, which takes less than units one after another).
-    const int units = ((a.q ? a.q_heads : 0) + a.kv_heads * (a.v ? 2 : 1)) * (D / 8);
-    const int threads = a.n >= 256 ? std::min(256, (units + 32 * lg::kRopeAhead - 1) / (32 * lg::kRopeAhead) * 32) : 128;
-    a.units_per_block = a.n >= 256 ? (units + 31) / 32 * 32 : threads;
-    a.parts = (units + a.units_per_block - 1) / a.units_per_block;
+template <typename In, typename Out, int D, int kLayout, int kTake>
+int launch_rope_pairs(lg::RopeRowsArgs& a, cudaStream_t st) {
+    const int items = ((a.q_heads + kTake - 1) / kTake + (a.kv_heads + kTake - 1) / kTake) * (D / 16);
+    a.parts = (items + 255) / 256;
+    const int threads = std::max(64, ((items + a.parts - 1) / a.parts + 31) / 32 * 32);
     const long long blocks = static_cast<long long>(a.n) * a.parts;
     if (blocks > INT32_MAX) return fail(LIGGUF_ATTN_EUNSUPPORTED, "%d tokens in one call", a.n);
-    lg::rope_rows_kernel<In, Out, D, kLayout><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
+    lg::rope_pairs_kernel<In, Out, D, kLayout, kTake><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
     LG_CUDA(cudaGetLastError());
     return LIGGUF_ATTN_OK;
 }
-
-// Prompts: the heads that are quantized by tiles of the cache, the others by rope_pairs_kernel beside it.
 template <typename In, typename Out, int D, int kLayout>
-int launch_rope_prompt(lg::RopeRowsArgs& a, cudaStream_t st) {
-    int device = 0, sms = 0;
-    LG_CUDA(cudaGetDevice(&device));
-    LG_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
-    if (a.tiles) {
-        const int tiles = (a.pos0 + a.n - 1) / lg::kKv4Tile - a.pos0 / lg::kKv4Tile + 1;
-        // Heads a block: as few as let all blocks be resident at once (a block's rotations serve all its heads).
-        const int slots = sms * lg::kKv4AppendBlocks;
-        a.kv_heads_per_block = std::min<long long>(a.kv_heads, (static_cast<long long>(tiles) * a.kv_heads + slots - 1) / slots);
-        a.kv_heads_per_block = std::max(a.kv_heads_per_block, 256 / (2 * D));
-        const int blocks = tiles * ((a.kv_heads + a.kv_heads_per_block - 1) / a.kv_heads_per_block);
-        lg::kv4_append_kernel<In, Out, D, kLayout><<<blocks, 256, 0, st>>>(a);
-        LG_CUDA(cudaGetLastError());
-    }
-    const int heads = (a.q ? a.q_heads : 0) + (a.tiles ? 0 : a.kv_heads);
-    if (heads == 0) return LIGGUF_ATTN_OK;
-    constexpr int take = sizeof(In) == 4 ? 1 : 2;
-    const int threads = std::min(256, ((heads + take - 1) / take * (D / 16) + 31) / 32 * 32);
-    auto kern = lg::rope_pairs_kernel<In, Out, D, kLayout>;
-    cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3(a.n);
-    lc.blockDim = dim3(threads);
-    lc.stream = st;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    lc.attrs = attr;
-    lc.numAttrs = a.tiles ? 1 : 0;  // beside kv4_append_kernel, which waited for what came before
-    LG_CUDA(cudaLaunchKernelEx(&lc, kern, a));
+int launch_rope_layout(lg::RopeRowsArgs& a, cudaStream_t st) {
+    if constexpr (kLayout != lg::kRopeHalvesOdd)
+        if (!a.tiles && a.n >= 32) return launch_rope_pairs<In, Out, D, kLayout, sizeof(In) == 4 ? 1 : 2>(a, st);
+    // Few tokens: their heads over several blocks, which take less time than a large one.
+    const int units = ((a.q ? a.q_heads : 0) + a.kv_heads * (a.v ? 2 : 1)) * (D / 8);
+    const int threads = a.n >= 128 ? 256 : 128;
+    a.units_per_block = a.n >= 128 ? (units + 31) / 32 * 32 : threads;
+    a.parts = (units + a.units_per_block - 1) / a.units_per_block;
+    const long long blocks = static_cast<long long>(a.n) * a.parts;
+    if (blocks > INT32_MAX) return fail(LIGGUF_ATTN_EUNSUPPORTED, "%d tokens in one call", a.n);
+    lg::rope_units_kernel<In, Out, D, kLayout><<<static_cast<unsigned>(blocks), threads, 0, st>>>(a);
+    LG_CUDA(cudaGetLastError());
     return LIGGUF_ATTN_OK;
 }
-
 template <typename In, typename Out, int D>
 int launch_rope_rows(lg::RopeRowsArgs& a, int layout, cudaStream_t st) {
-    // By tiles and pairs from 64 tokens on: below, their blocks are too few and the byte-wise form is as fast.
-    if (layout == lg::kRopeHalvesOdd) return launch_rope_units<In, Out, D, lg::kRopeHalvesOdd>(a, st);
-    if (layout == lg::kRopeAdjacent)
-        return a.n >= 64 ? launch_rope_prompt<In, Out, D, lg::kRopeAdjacent>(a, st)
-                         : launch_rope_units<In, Out, D, lg::kRopeAdjacent>(a, st);
-    return a.n >= 64 ? launch_rope_prompt<In, Out, D, lg::kRopeHalves>(a, st)
-                     : launch_rope_units<In, Out, D, lg::kRopeHalves>(a, st);
+    if (layout == lg::kRopeHalvesOdd) return launch_rope_layout<In, Out, D, lg::kRopeHalvesOdd>(a, st);
+    return layout == lg::kRopeAdjacent ? launch_rope_layout<In, Out, D, lg::kRopeAdjacent>(a, st)
+                                       : launch_rope_layout<In, Out, D, lg::kRopeHalves>(a, st);
 }
 template <typename In, typename Out>
 int launch_rope_rows_d(lg::RopeRowsArgs& a, const ligguf_rope_cfg& r, cudaStream_t st) {
