@@ -460,10 +460,10 @@ __device__ __forceinline__ TcWinItem tc_window_item(const TcArgs& a, int idx, in
     it.b = idx / (a.q_heads * n_qt);
     it.r0 = (n_qt - 1 - y) * kTcRows;
     it.nq_valid = a.q_seq;
-    it.kv_len = a.lens ? max(0, min(a.lens[it.b], a.kv_seq)) : a.kv_seq;
+    it.kv_len = a.lens ? max(0, min(__ldg(a.lens + it.b), a.kv_seq)) : a.kv_seq;
     // A first position below -q_seq (nothing is seen) or beyond every key and window (only first tokens
     // are) gives what the nearest bound gives; the bounds keep the sums below 2^31.
-    const int first = a.pos0 ? a.pos0[it.b] : it.kv_len - a.q_seq;
+    const int first = a.pos0 ? __ldg(a.pos0 + it.b) : it.kv_len - a.q_seq;
     it.p0 = max(-a.q_seq, min(first, a.kv_seq + a.window)) + it.r0;
     const int p1 = it.p0 + min(kTcRows, a.q_seq - it.r0) - 1;
     it.hi = max(0, min(it.kv_len, p1 + 1));
