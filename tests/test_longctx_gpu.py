@@ -559,3 +559,109 @@ def test_empty_calls_do_nothing(gpu):
     h.attn_async(1, 2, 0, q, None, None, out)  # no keys at all: zeros
     h.status()
     assert not out.any()
+
+
+# ------------------------------------------------------------------------------- calls that are refused
+def test_calls_with_bad_arguments_are_refused(gpu):
+    """Each of these returns before anything is launched."""
+    import torch
+    from ligguf_b200 import LigGufAttnError, QkRope, QkRopeConfig, RopeConfig, WindowAttention, WindowConfig
+    x = torch.zeros(4096, device="cuda")
+    h = x.half()
+    odd = x[1:]  # 4 bytes past an aligned address
+    rope = RopeConfig(64, 64)
+    r = QkRope(QkRopeConfig(rope=rope, n_heads=1, n_kv_heads=1, qk_norm=True))
+    c = make_cache(64, 1, 1, n_context=16, n_seqs=2, qk_norm=True)
+    w = WindowAttention(WindowConfig(1, 1, 64, in_type=F16, out_type=F16))
+
+    def refused(status, word, f, *a, **k):
+        with pytest.raises(LigGufAttnError, match=word) as e:
+            f(*a, **k)
+        assert e.value.status == status
+
+    bad, state = _lib.EINVAL, _lib.ESTATE
+    refused(bad, "tokens", r.run_async, -1, x, x, x, x)
+    refused(bad, "tokens", r.run_async, 2, x, x, x, x, pos0=2 ** 31 - 2)
+    refused(bad, "null", r.run_async, 1, None, x, x, x)
+    refused(bad, "null", r.run_async, 1, x, x, x, None)
+    refused(bad, "norm weights", r.run_async, 1, x, x, x, x, q_gamma=x)
+    refused(bad, "aligned", r.run_async, 1, odd, x, x, x, q_gamma=x, k_gamma=x)
+    refused(state, "were not set", c.append_async, 0, 0, 0, 1, None, x, x)
+    refused(state, "were not set", c.decode_async, 0, 1, x, x, x, x)
+    g = np.ones(64, np.float32)
+    with pytest.raises(ValueError):
+        c.set_qk_norm(0, g[:32], g)
+    refused(bad, "layer", c.set_qk_norm, 1, g, g)
+    c.set_qk_norm(0, g, g)
+    refused(bad, "layer", c.append_async, -1, 0, 0, 1, None, x, x)
+    refused(bad, "sequences", c.append_async, 0, 2, 0, 1, None, x, x)
+    refused(bad, "positions", c.append_async, 0, 0, 15, 2, None, x, x)
+    refused(bad, "positions", c.append_async, 0, 0, 0, -1, None, x, x)
+    refused(bad, "null", c.append_async, 0, 0, 0, 1, None, x, None)
+    refused(bad, "null", c.append_async, 0, 0, 0, 1, None, x, x, x)  # queries wanted, none given
+    refused(bad, "aligned", c.append_async, 0, 0, 0, 1, None, odd, x)
+    refused(bad, "sequences", c.decode_async, 0, 3, x, x, x, x)
+    refused(bad, "pos", c.decode_async, 0, 1, x, x, x, x, pos=16)
+    refused(bad, "pos", c.decode_async, 0, 1, x, x, x, x, pos=-1)
+    refused(bad, "null", c.decode_async, 0, 1, x, x, None, x)
+    refused(bad, "aligned", c.decode_async, 0, 1, x, x, x, odd)
+    refused(bad, "positions", c.read_async, 0, 0, 10, 7, x, x)
+    refused(bad, "sequences", c.load_async, 0, 1, 2, 0, 1, x, x)
+    refused(bad, "null", c.store_async, 0, 0, 1, 0, 1, x, None)
+    refused(bad, "batch", w.attn_async, -1, 1, 1, h, h, h, h)
+    refused(bad, "batch", w.attn_async, 1, 1, 1 << 30, h, h, h, h)
+    refused(bad, "null", w.attn_async, 1, 1, 1, h, None, h, h)
+    refused(bad, "aligned", w.attn_async, 1, 1, 1, h, h[1:], h, h)
+    c.status()
+    w.status()
+
+
+def test_cache_beyond_the_memory_is_refused(gpu):
+    from ligguf_b200 import LigGufAttnError
+    for seqs, status in ((2048, _lib.ENOMEM), (65535, _lib.EUNSUPPORTED)):
+        with pytest.raises(LigGufAttnError) as e:
+            make_cache(128, 8, 4, n_context=1 << 20, n_seqs=seqs, n_layers=64)
+        assert e.value.status == status
+
+
+def test_kv4_offsets_beyond_32_bits(gpu):
+    """The last layer of a cache of 5.7 GB: tiles past 2^32 bytes, and the last positions of a context of 2^18."""
+    rng = np.random.default_rng(12)
+    n = 1 << 18
+    c = make_cache(128, 8, 1, n_context=n, n_layers=9, window=200, sinks=3, rows_type=F32)
+    g = 300
+    kb, vb = (ref.q40(rng.standard_normal((1, g, 8 * 128))) for _ in range(2))
+    first = n - g
+    c.load_async(8, 0, 1, first, g, dev(kb), dev(vb))
+    assert np.array_equal(store(c, 8, 0, 1, first, g)[1], vb)
+    q, dq = rounded(rng.standard_normal((1, 8, 128)), F32)
+    k, dk = rounded(rng.standard_normal((1, 8, 128)), F32)
+    v, dv = rounded(rng.standard_normal((1, 8, 128)), F32)
+    import torch
+    out = torch.empty(1, 8 * 128, device="cuda")
+    c.decode_async(8, 1, dq, dk, dv, out, pos=n - 1)
+    freq = ref.frequencies(128, 1e4)
+    qr, kr = (ref.rotate(x, [n - 1], freq, "adjacent") for x in (q, k))
+    keys = ref.seen(n - 1, n - 1, 200, 0)  # the first tokens are zeros: keys of score 0, values of 0
+    want = np.zeros((8, 128))
+    kk = ref.q40_values(kb[0, keys - first]).reshape(-1, 8, 128)
+    vv = ref.q40_values(vb[0, keys - first]).reshape(-1, 8, 128)
+    for h in range(8):
+        zero = np.zeros((3, 128))
+        want[h] = ref.attend(qr[0, h], np.concatenate([zero, kk[:, h], kr[0, h][None]]),
+                             np.concatenate([zero, vv[:, h], v[0, h][None]]), 128 ** -0.5)
+    close(host(out).reshape(8, 128), want, 2e-5 * np.abs(want).max())
+
+
+def test_example_runs_the_operators_together(gpu):
+    """examples/long_context.py: prompt and draft within the operands' rounding (2^-8 of bf16, weights and exponentials
+    as for windowed attention: 1.1e-4 + 2^-8 of the largest value, twice for values and result of unlike size), single
+    tokens within fp32's."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "long_context.py")
+    spec = importlib.util.spec_from_file_location("long_context", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    e = m.run(prompt=1300, chunk=555, tokens=3, window=400)
+    assert e["prompt"] <= 1e-2 and e["draft"] <= 1e-2 and e["tokens"] <= 2e-5, e
