@@ -894,8 +894,9 @@ __global__ void __launch_bounds__(32 * kv4_warps(NREP), kv4_blocks_per_sm(NREP))
         if (!*last) return;
         const float* parts = a.parts + static_cast<long long>(e.first) * 2 * PF;
         auto part = [&](int w) { return parts + (w ? w * 2 : e.lead) * PF; };
-        // Threads in groups, one 16-byte column a thread; a group takes every kGroups-th part.
-        constexpr int kCols = NREP * D / 4, kGroups = kThreads / kCols, kAhead = 8;
+        // Threads in groups, one 16-byte column a thread; a group takes every kGroups-th part.  All loads leave at
+        // once, for up to kGroups * kAhead parts: one trip to the L2 instead of several.
+        constexpr int kCols = NREP * D / 4, kGroups = kThreads / kCols, kAhead = 20;
         const int col = threadIdx.x % kCols, grp = threadIdx.x / kCols;
         float4 y8[kAhead];
 #pragma unroll
@@ -904,14 +905,23 @@ __global__ void __launch_bounds__(32 * kv4_warps(NREP), kv4_blocks_per_sm(NREP))
         float* inv = reinterpret_cast<float*>(smem + Sm::kFactors);
         float* fac = inv + NREP;
         for (int h = warp; h < NREP; h += kWarps) {  // the parts' factors, a head a warp
-            float m0 = -1e30f, l0 = 0.f;  // of part `lane`, which is all of them up to 32
-            if (lane < e.parts) m0 = __ldcg(part(lane) + NREP * D + h), l0 = __ldcg(part(lane) + NREP * D + NREP + h);
-            float M = m0;
-            for (int w = lane + 32; w < e.parts; w += 32) M = fmaxf(M, __ldcg(part(w) + NREP * D + h));
-            M = warp_max(M);
-            float l = l0 * ex2(m0 - M);
-            if (lane < e.parts) fac[lane * NREP + h] = ex2(m0 - M);
-            for (int w = lane + 32; w < e.parts; w += 32) {
+            float m2[2], l2[2], M = -1e30f;  // of parts `lane` and `lane` + 32, which is all of them up to 64
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const int w = lane + 32 * u;
+                m2[u] = w < e.parts ? __ldcg(part(w) + NREP * D + h) : -1e30f;
+                l2[u] = w < e.parts ? __ldcg(part(w) + NREP * D + NREP + h) : 0.f;
+            }
+            for (int w = lane + 64; w < e.parts; w += 32) M = fmaxf(M, __ldcg(part(w) + NREP * D + h));
+            M = warp_max(fmaxf(M, fmaxf(m2[0], m2[1])));
+            float l = 0.f;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const float f = ex2(m2[u] - M);
+                if (lane + 32 * u < e.parts) fac[(lane + 32 * u) * NREP + h] = f;
+                l = fmaf(l2[u], f, l);
+            }
+            for (int w = lane + 64; w < e.parts; w += 32) {
                 const float f = ex2(__ldcg(part(w) + NREP * D + h) - M);
                 fac[w * NREP + h] = f;
                 l = fmaf(__ldcg(part(w) + NREP * D + NREP + h), f, l);
