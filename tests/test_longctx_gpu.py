@@ -371,6 +371,54 @@ def test_kv4_decode_mixed_value_magnitudes_and_large_scores(gpu):
     close(out, want, 1e-4 * np.abs(want).max())
 
 
+@pytest.mark.parametrize("rows,dim,Hk,nrep", [(33, 64, 1, 2), (100, 128, 2, 4), (7, 64, 40, 1), (40, 64, 33, 2)])
+def test_kv4_decode_many_rows_and_heads(gpu, rows, dim, Hk, nrep):
+    """More sequences and KV heads than a warp has lanes, idle ones among them; from the device and, with one position
+    for all, from the host."""
+    rng = np.random.default_rng(rows)
+    pos = rng.integers(-2, 150, rows)
+    c = make_cache(dim, Hk, nrep, n_context=150, n_seqs=rows, window=70, sinks=2)
+    kb, vb, qkv, d = decode_case(rng, c, pos, F32)
+    out, kr, vr = run_decode(c, d, pos, F32)
+    want = decode_ref(c, kb, vb, qkv, pos)
+    close(out, want, 2e-5 * np.abs(want).max())
+    assert not out[pos < 0].any()
+    check_rows(c, pos[:40], kr, vr)
+    c.load_async(0, 0, rows, 0, 150, dev(kb), dev(vb))
+    pos = np.full(rows, 149)
+    out, _, _ = run_decode(c, d, pos, F32, device_pos=False)
+    want = decode_ref(c, kb, vb, qkv, pos)
+    close(out, want, 2e-5 * np.abs(want).max())
+
+
+@pytest.mark.parametrize("rope_dim,layout", [(20, "halves"), (48, "halves"), (62, "adjacent"), (2, "halves")])
+@pytest.mark.parametrize("n", [3, 200])
+def test_kv4_partly_rotated_heads(gpu, rope_dim, layout, n):
+    """Rotated parts that are not whole units of eight elements, appended and decoded."""
+    import torch
+    rng = np.random.default_rng(rope_dim)
+    c = make_cache(64, 2, 2, n_context=n + 1, rope_dim=rope_dim, layout=layout, rows_type=F32)
+    x, dx = rounded(rng.standard_normal((n, 8 * 64)), F32)
+    q, k, v = (x[:, a:b].reshape(n, -1, 64) for a, b in ((0, 256), (256, 384), (384, 512)))
+    qo, kr, vr = (torch.empty(n, w, device="cuda") for w in (256, 128, 128))
+    c.append_async(0, 0, 0, n, *(dx[:, a:b].contiguous() for a, b in ((0, 256), (256, 384), (384, 512))), qo, kr, vr)
+    freq = ref.frequencies(rope_dim, 1e4)
+    want = ref.rotate(q, np.arange(n), freq, layout)
+    close(host(qo).reshape(want.shape), want, 1e-5 * np.abs(want).max())
+    kb, vb = store(c, 0, 0, 1, 0, n)
+    yk = ref.rotate(k, np.arange(n), freq, layout).reshape(n, -1, 32)
+    d = np.abs(np.ascontiguousarray(kb[0, ..., :2]).view(np.float16).astype(np.float64))
+    top = np.concatenate([kb[0, ..., 2:] & 15, kb[0, ..., 2:] >> 4], -1) == 15
+    assert (np.abs(ref.q40_values(kb[0]).reshape(yk.shape) - yk) <= d * np.where(top, 1.01, 0.505)).all()
+    assert np.array_equal(vb[0], ref.q40(v.reshape(n, -1)))
+    kb, vb = (np.concatenate([b, np.zeros((1, 1) + b.shape[2:], np.uint8)], 1) for b in (kb, vb))
+    qkv = [x for x in (rng.standard_normal((1, 4, 64)), rng.standard_normal((1, 2, 64)), rng.standard_normal((1, 2, 64)))]
+    qkv, dd = zip(*(rounded(x, F32) for x in qkv))
+    out, _, _ = run_decode(c, dd, [n], F32)
+    want = decode_ref(c, kb, vb, qkv, [n])
+    close(out, want, 2e-5 * np.abs(want).max())
+
+
 def test_kv4_decode_poisoned_unseen_rows(gpu):
     """NaN in rows that the window hides, beyond the position, and in the token's own old row."""
     rng = np.random.default_rng(6)
