@@ -158,11 +158,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
         const bool edge = k0 + kFewKeys > sp.p0 + 1 || k0 + kFewKeys > sp.hi || (k0 < sp.lo + a.n && a.window);
         if (k0 + kFewKeys > sp.hi || (k0 < sp.lo && k0 + kFewKeys > a.sinks)) {
             // Rows of V that no query sees may hold anything, and 0 * NaN is NaN.
-            for (int r = threadIdx.x; r < kFewKeys; r += 32 * kFewWarps) {
+            for (int r = threadIdx.x >> 3; r < kFewKeys; r += 4 * kFewWarps) {
                 if (k0 + r < sp.hi && (k0 + r >= sp.lo || k0 + r < a.sinks)) continue;
                 for (int c = 0; c < D / 64; ++c)
-                    for (int i = 0; i < 8; ++i)
-                        *reinterpret_cast<uint4*>(tile + Sm::kTile + c * Sm::kChunk + r * 128 + i * 16) = make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4*>(tile + Sm::kTile + c * Sm::kChunk + r * 128 + (threadIdx.x & 7) * 16) = make_uint4(0, 0, 0, 0);
             }
             fence_proxy_async_smem();  // before a later copy into these rows
             __syncthreads();
