@@ -197,6 +197,9 @@ struct TcTmem {
     static_assert(kO + 2 * D <= kTcTmemCols, "TMEM plan exceeds 512 columns");
 };
 
+// Windowed form: items of a CTA that are worked out once, at its start, by as many threads; the roles read them (an
+// item takes divisions and two loads, which every role would wait for between two items).
+constexpr int kTcItems = 64, kTcItemInts = 11;
 template <int D>
 struct TcSmem {
     static constexpr int kChunks = D / 64;               // 128-byte column chunks of a row
@@ -221,7 +224,8 @@ struct TcSmem {
     // q_empty[2], o_final[2], o_free[2], l_full[kLRing]
     static constexpr int kNumBars = 4 * kStages + 2 + 2 + 2 + 1 + 8 + kLRing + 8 + 2;  // + xchg[2][4], v_ask, v_fixed
     static constexpr size_t kMisc = kBar + size_t(kNumBars) * 8;  // tmem base, abort flag
-    static constexpr size_t kTotal = kMisc + 16 + 1024;           // + slack to align the base to 1 KB
+    static constexpr size_t kItems = kMisc + 16;                  // windowed: this CTA's first items, worked out ahead
+    static constexpr size_t kTotal = kItems + size_t(kTcItems) * kTcItemInts * 4 + 1024;  // + slack to align the base to 1 KB
 };
 
 // ------------------------------------------------------------------------------ tcgen05 wrappers
@@ -483,10 +487,11 @@ __device__ __forceinline__ int tc_window_key0(const TcWinItem& it, int j) {
 __device__ __forceinline__ bool tc_window_fix(const TcArgs& a, const TcWinItem& it, int k0) {
     return k0 + kTcKeys > it.hi || (k0 < it.lo && k0 + kTcKeys > a.sinks);
 }
+static_assert(sizeof(TcWinItem) == kTcItemInts * 4, "the items' room in shared memory");
 template <typename Mode>
-__device__ __forceinline__ auto tc_any_item(const TcArgs& a, int idx, int n_qt) {
+__device__ __forceinline__ auto tc_any_item(const TcArgs& a, const void* items, int w, int idx, int n_qt) {
     if constexpr (Mode::kWindow)
-        return tc_window_item(a, idx, n_qt);
+        return w < kTcItems ? static_cast<const TcWinItem*>(items)[w] : tc_window_item(a, idx, n_qt);
     else
         return tc_item(a, idx, n_qt);
 }
@@ -588,6 +593,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     // access below comes after that grid has completed.  This kernel does not trigger its own
     // dependents early: they launch when it exits.
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    const void* items = sm + Sm::kItems;
+    if constexpr (kWin) {
+        if (threadIdx.x < kTcItems) {
+            const int idx = tc_walk(a, threadIdx.x, n_items);
+            if (idx >= 0) reinterpret_cast<TcWinItem*>(sm + Sm::kItems)[threadIdx.x] = tc_window_item(a, idx, n_qt);
+        }
+        __syncthreads();
+    }
 
     if (warp < 4) {
         reg_set<kTcRegsIssue>();
@@ -600,7 +613,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int w = 0; ok; ++w) {
                     const int idx = tc_walk(a, w, n_items);
                     if (idx < 0) break;
-                    const auto it = tc_any_item<Mode>(a, idx, n_qt);
+                    const auto it = tc_any_item<Mode>(a, items, w, idx, n_qt);
                     if (it.n_kv == 0) continue;
                     deadline = globaltimer_ns() + kWaitLimitNs;
                     // Q of item z into buffer z & 1, once the last S MMA of item z - 2 has read it.
@@ -672,7 +685,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int w = 0; ok; ++w) {
                     const int idx = tc_walk(a, w, n_items);
                     if (idx < 0) break;
-                    const auto it = tc_any_item<Mode>(a, idx, n_qt);
+                    const auto it = tc_any_item<Mode>(a, items, w, idx, n_qt);
                     const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
                     for (int j = 0; j < it.n_kv; ++j, ++t) {
                         const int s = t % S, k0 = tc_window_key0(it, j);
@@ -717,7 +730,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 for (int w = 0; ok; ++w) {
                     const int idx = tc_walk(a, w, n_items);
                     if (idx < 0) break;
-                    const auto it = tc_any_item<Mode>(a, idx, n_qt);
+                    const auto it = tc_any_item<Mode>(a, items, w, idx, n_qt);
                     const int n_kv = it.n_kv;
                     if (n_kv == 0) continue;
                     deadline = globaltimer_ns() + kWaitLimitNs;
@@ -813,7 +826,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int w = 0; ok; ++w) {
             const int idx = tc_walk(a, w, n_items);
             if (idx < 0) break;
-            const auto it = tc_any_item<Mode>(a, idx, n_qt);
+            const auto it = tc_any_item<Mode>(a, items, w, idx, n_qt);
             if (it.n_kv == 0) continue;
             const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
             const int qr = it.r0 + row;  // query row within the sequence
@@ -967,7 +980,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         for (int w = 0; ok; ++w) {
             const int idx = tc_walk(a, w, n_items);
             if (idx < 0) break;
-            const auto it = tc_any_item<Mode>(a, idx, n_qt);
+            const auto it = tc_any_item<Mode>(a, items, w, idx, n_qt);
             const int row0 = it.r0 + quarter * 32;  // first sequence row of this warp's 32 rows
             using Out = typename Mode::Out;
             Out* obase = (kWin ? static_cast<Out*>(a.wout) : reinterpret_cast<Out*>(a.out)) +
