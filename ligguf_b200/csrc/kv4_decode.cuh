@@ -9,10 +9,10 @@
 // from the packed codes:
 //   - Keys: a code n (0..15) masked into the low mantissa bits of a half is the subnormal n * 2^-24, and
 //     shifted by a nibble n * 2^-20: exact operands that cost one AND for two codes.  The powers of two are
-//     taken out of the fp32 results, and the -8 of (n - 8) d is added to a group's sum.  The
-//     tensor cores align products by their operands' exponent fields and cut off what lies 24 bits below the
-//     largest, and a subnormal's field is that of 2^-14: so the queries' hi parts are whole numbers, which
-//     makes every product and sum of hi parts exact, cut or not.
+//     taken out of the fp32 results, and the -8 of (n - 8) d is added to a group's sum.  The tensor cores
+//     align products by their operands' exponent fields and cut off what lies 24 bits below the largest, and
+//     a subnormal's field is that of 2^-14: so the queries' hi parts are whole numbers, which makes every
+//     product and sum of hi parts exact, cut or not.
 //   - Values: the weights cannot be whole numbers, and with subnormal codes that cut costs 7 bits (results
 //     were off by 9e-6).  So 0x6400 is OR-ed in by the same instruction (1024 + n, or 1024 + 16 n), and one
 //     packed subtraction (or multiply-add) makes it n - 8: normal halves, exact as well.
@@ -34,8 +34,8 @@
 // one unit for the token itself, cut into equal contiguous shares of as many blocks as fit at once, whatever
 // the lengths of the sequences; the cut is computed by every block from the positions, which may be in
 // device memory.  In a share, the 8 warps take pairs of tiles in turn, each with its own ring of bulk copies
-// and its own running sums, which the block joins per item.  Items that several blocks share are joined by the last of them to
-// finish, in the order of the blocks, so results repeat bit for bit.
+// and its own running sums, which the block joins per item.  Items that several blocks share are joined by
+// the last of them to finish, in the order of the blocks, so results repeat bit for bit.
 #pragma once
 
 #include "kv4.cuh"
@@ -70,9 +70,11 @@ enum : int { KERR_POSITION = 16 };
 __host__ __device__ constexpr int kv4_warps(int) { return 8; }
 __host__ __device__ constexpr int kv4_blocks_per_sm(int nrep) { return nrep > 4 ? 1 : 2; }
 // Units that an item counts beside its tiles and its token: what a block spends on entering and joining an
-// item, in tiles (24 to 72 measured: 16 streams of 4100 tiles 33.0, 32.2, 31.6, 31.4 us, 24 sequences 44.6, 44.3, 44.0, 44.4).
+// item, in tiles (24, 40, 56, 72: 16 streams of 4100 positions 33.0, 32.2, 31.6, 31.4 us, 24 sequences up to 8191
+// 44.6, 44.3, 44.0, 44.4 us).
 constexpr int kKv4ItemUnits = 56;
-// Units a block has at least: an item is not cut up for fewer tiles than the join of its parts costs.
+// Units a block has at least: with fewer, a short context's join takes longer than its tiles (512 positions of four
+// KV heads: 8.8 us with 16, 9.3 with 24, 13 with 96, where one block takes a head).
 constexpr int kKv4MinUnits = 16;
 
 // Floats of one partial result: o [NREP][D], m [NREP], l [NREP], in whole 16 bytes.
