@@ -388,15 +388,18 @@ int launch_window_few(const ligguf_window* h, const lg::WindowArgs& w, cudaStrea
     }
     lg::WindowFewArgs f = {};
     f.w = w;
+    f.tokens = std::min(w.n, lg::kFewRows / (w.q_heads / w.kv_heads));
+    f.chunks = (w.n + f.tokens - 1) / f.tokens;
     f.parts = h->parts;
     f.err = h->d_err;
-    // Splits: one wave of two CTAs an SM, at least two tiles each.
-    const long long pairs = static_cast<long long>(w.batch) * w.kv_heads;
+    // Splits: one wave of two CTAs an SM, at least two tiles each (4 tokens over 16448 keys: 19.2 us; with one CTA
+    // an SM 20.8, or 22.1 with a ring of three tiles; with 1.5 20.1).
+    const long long pairs = static_cast<long long>(w.batch) * f.chunks * w.kv_heads;
     const long long keys = w.window ? std::min<long long>(w.m, static_cast<long long>(w.window) + w.n + w.sinks + 2 * lg::kFewKeys) : w.m;
     const long long tiles = (keys + lg::kFewKeys - 1) / lg::kFewKeys;
     f.splits = static_cast<int>(std::max(1ll, std::min(few_most_items(h->num_sms) / pairs, (tiles + 1) / 2)));
     cudaLaunchConfig_t lc = {};
-    lc.gridDim = dim3(f.splits, w.kv_heads, w.batch);
+    lc.gridDim = dim3(f.splits, w.kv_heads * f.chunks, w.batch);
     lc.blockDim = dim3(32 * lg::kFewWarps);
     lc.dynamicSmemBytes = lg::FewSmem<D>::kTotal;
     lc.stream = st;
@@ -417,9 +420,22 @@ int launch_window_few(const ligguf_window* h, const lg::WindowArgs& w, cudaStrea
 template <typename T, typename Out, int D>
 int launch_window_d(const ligguf_window* h, const lg::WindowArgs& a, cudaStream_t st) {
     // Few rows a KV head: all of them against each key tile once, the keys split over the SMs.  Up to 64 rows this
-    // is bound by K and V; the tensor-core form reads them once a head and gives a head's keys to one SM.
-    const int rows = a.n * (a.q_heads / a.kv_heads);
-    if (rows <= lg::kFewRows && a.batch <= 65535 && a.kv_heads <= 65535) {
+    // is bound by K and V; the tensor-core form reads them once a head and gives a head's keys to one SM.  More rows
+    // go in chunks of 64 where the tensor-core form would leave most SMs without work: one of its SMs takes about
+    // 9 us for 1024 keys of a head, a chunk 20 us of one SM's time, and there is a join.  Hence the bounds of a
+    // quarter as many chunks as SMs and of 1024 keys.  Measured, 32 heads and 8 KV heads of 128, one sequence, us in
+    // chunks / on the tensor cores: 17 tokens, 512 keys 10.4 / 10.6, 1024 11.4 / 14.9, 4096 22.4 / 41.2, 32768
+    // 76.6 / 297; 64 tokens, 512 keys 12.7 / 10.7, 1024 15.2 / 15.2, 32768 135 / 297; 100 tokens (56 chunks), 2048
+    // keys 27.9 / 24.2, 32768 231 / 297.
+    const int nrep = a.q_heads / a.kv_heads;
+    const long long rows = static_cast<long long>(a.n) * nrep;
+    const long long keys = a.window ? std::min<long long>(a.m, static_cast<long long>(a.window) + a.n + a.sinks) : a.m;
+    bool few = rows <= lg::kFewRows;
+    if (!few && nrep <= lg::kFewRows && keys >= 1024) {
+        const long long tokens = lg::kFewRows / nrep, chunks = (a.n + tokens - 1) / tokens;
+        few = chunks * a.batch * a.kv_heads <= h->num_sms / 4;
+    }
+    if (few && a.batch <= 65535 && a.kv_heads <= 65535) {
         if (rows <= 16) return launch_window_few<T, Out, D, 1>(h, a, st);
         return rows <= 32 ? launch_window_few<T, Out, D, 2>(h, a, st) : launch_window_few<T, Out, D, 4>(h, a, st);
     }

@@ -16,35 +16,36 @@ struct WindowArgs {
 };
 
 // ---------------------------------------------------------------------------- few query rows
-// The rows of one KV head's queries (n tokens x n_heads/n_kv_heads heads, at most 64) against long runs of
-// keys: bound by the bytes of K and V, which every CTA reads once for all of its rows.
+// The rows of one KV head's queries (tokens x n_heads/n_kv_heads heads, at most 64) against long runs of keys: bound
+// by the bytes of K and V, which every CTA reads once for all of its rows.  More tokens go in chunks of at most 64
+// rows, each over its own visible tiles (then bound by the matrix instructions).
 //
-// Grid (split, KV head, batch entry): a CTA takes an equal run of the entry's visible key tiles (64 keys; the
-// run is worked out from pos0 and lens, which lie in device memory) and leaves its rows' unnormalised sums,
-// maxima and row sums; window_join_kernel adds the splits up, in order.  The four warps are row groups of 16
-// rows x parts of the tile's keys.  K and V tiles come by TMA into a ring of two (SWIZZLE_128B rows of 64
-// columns), S = Q K^T and O += P V run on mma.m16n8k16 with ldmatrix reading the swizzled rows; S of a warp is
-// P's operand without any exchange.  (tcgen05 wants 128 rows; with 16 of them in use its tiles would be mostly
-// padding, and the kernel is bound by memory either way.)
+// Grid (split, KV head and chunk, batch entry): a CTA takes an equal run of its visible key tiles (64 keys; the run
+// is worked out from pos0 and lens, which lie in device memory) and leaves its rows' unnormalised sums, maxima and
+// row sums; window_join_kernel adds the splits up, in order.  The four warps are row groups of 16 rows x parts of
+// the tile's keys.  K and V tiles come by TMA into a ring of two (SWIZZLE_128B rows of 64 columns), S = Q K^T and
+// O += P V run on mma.m16n8k16 with ldmatrix reading the swizzled rows; S of a warp is P's operand without any
+// exchange.  (tcgen05 wants 128 rows; with 16 of them in use its tiles would be mostly padding, and the kernel is
+// bound by memory either way.)
 constexpr int kFewKeys = 64, kFewWarps = 4, kFewStages = 2, kFewRows = 64;
 
 struct WindowFewArgs {
     WindowArgs w;
-    int splits;
-    float* parts;  // [entry][KV head][split][rows][D + 2]: o, then m, then l (m in log2 units)
+    int splits, tokens, chunks;  // tokens of a chunk
+    float* parts;  // [entry][chunk][KV head][split][rows][D + 2]: o, then m, then l (m in log2 units)
     int* err;
 };
 
-// The visible key tiles of an entry's rows: tiles [0, ns) of the first tokens, then [tw, tw + nt - ns).
+// The visible key tiles of tokens [i0, i0 + n) of an entry: tiles [0, ns) of the first tokens, then [tw, tw + nt - ns).
 struct FewSpan {
     int p0, lo, hi, ns, tw, nt;
 };
-__device__ __forceinline__ FewSpan few_span(const WindowArgs& a, int b) {
+__device__ __forceinline__ FewSpan few_span(const WindowArgs& a, int b, int i0, int n) {
     FewSpan f;
     const int len = a.lens ? max(0, min(a.lens[b], a.m)) : a.m;
     // (bounded as in tc_window_item: positions beyond every key and window are all alike)
-    f.p0 = max(-a.n, min(a.pos0 ? a.pos0[b] : len - a.n, a.m + a.window));
-    f.hi = max(0, min(len, f.p0 + a.n));
+    f.p0 = max(-a.n, min(a.pos0 ? a.pos0[b] : len - a.n, a.m + a.window)) + i0;
+    f.hi = max(0, min(len, f.p0 + n));
     f.lo = a.window ? max(0, min(f.p0 - a.window + 1, f.hi)) : 0;
     const int te = (f.hi + kFewKeys - 1) / kFewKeys, sinks = a.window ? min(a.sinks, f.hi) : 0;
     f.tw = min(f.lo / kFewKeys, te);
@@ -104,8 +105,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
     const WindowArgs& a = f.w;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int group = warp % kGroups, part = warp / kGroups;
-    const int split = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
-    const int nrep = a.q_heads / a.kv_heads, rows = a.n * nrep;
+    const int split = blockIdx.x, head = blockIdx.y % a.kv_heads, chunk = blockIdx.y / a.kv_heads, b = blockIdx.z;
+    const int i0 = chunk * f.tokens, n = min(f.tokens, a.n - i0), nrep = a.q_heads / a.kv_heads, rows = n * nrep;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kFewStages; ++s) mbar_init(&full[s], 1);
         *abort = 0;
@@ -115,7 +116,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
-    const FewSpan sp = few_span(a, b);
+    const FewSpan sp = few_span(a, b, i0, n);
     const int t0 = static_cast<int>(static_cast<long long>(sp.nt) * split / f.splits);
     const int t1 = static_cast<int>(static_cast<long long>(sp.nt) * (split + 1) / f.splits);
     auto key0 = [&](int i) { return (i < sp.ns ? i : sp.tw + (i - sp.ns)) * kFewKeys; };
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
     for (int u = 0; u < 2; ++u) {
         const int r = group * 16 + g + 8 * u, i = r / nrep;
         p[u] = r < rows ? sp.p0 + i : -1;  // a row that is not there sees nothing
-        const T* q = static_cast<const T*>(a.q) + b * a.q_batch + static_cast<long long>(i) * a.q_stride + (head * nrep + r % nrep) * D;
+        const T* q = static_cast<const T*>(a.q) + b * a.q_batch + static_cast<long long>(i0 + i) * a.q_stride + (head * nrep + r % nrep) * D;
 #pragma unroll
         for (int j = 0; j < KS; ++j) {
             qa[j][u] = r < rows ? *reinterpret_cast<const uint32_t*>(q + 16 * j + 2 * t) : 0u;
@@ -155,7 +156,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
             *reinterpret_cast<volatile int*>(f.err) = KERR_TIMEOUT_FULL;
         }
         uint8_t* tile = smem + Sm::kRing + s * 2 * Sm::kTile;
-        const bool edge = k0 + kFewKeys > sp.p0 + 1 || k0 + kFewKeys > sp.hi || (k0 < sp.lo + a.n && a.window);
+        const bool edge = k0 + kFewKeys > sp.p0 + 1 || k0 + kFewKeys > sp.hi || (k0 < sp.lo + n && a.window);
         if (k0 + kFewKeys > sp.hi || (k0 < sp.lo && k0 + kFewKeys > a.sinks)) {
             // Rows of V that no query sees may hold anything, and 0 * NaN is NaN.
             for (int r = threadIdx.x >> 3; r < kFewKeys; r += 4 * kFewWarps) {
@@ -245,8 +246,8 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
         if (t == 0) sm[warp * 16 + g + 8 * u] = m[u], sl[warp * 16 + g + 8 * u] = l[u];
     }
     __syncthreads();
-    const long long item = (static_cast<long long>(b) * a.kv_heads + head) * f.splits + split;
-    float* parts = f.parts + item * rows * (D + 2);
+    const long long item = ((static_cast<long long>(b) * f.chunks + chunk) * a.kv_heads + head) * f.splits + split;
+    float* parts = f.parts + item * (f.tokens * nrep) * (D + 2);
     for (int i = threadIdx.x; i < rows * (D / 4); i += 32 * kFewWarps) {
         const int r = i / (D / 4), d = i % (D / 4) * 4, w0 = r / 16, rr = r % 16;
         float M = -INFINITY, ls = 0.f;
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
         }
         if (f.splits == 1) {
             const float inv = ls != 0.f ? 1.f / ls : 0.f;
-            Out* out = static_cast<Out*>(a.out) + ((static_cast<long long>(b) * a.n + r / nrep) * a.q_heads + head * nrep + r % nrep) * D + d;
+            Out* out = static_cast<Out*>(a.out) + ((static_cast<long long>(b) * a.n + i0 + r / nrep) * a.q_heads + head * nrep + r % nrep) * D + d;
             tc_store4(out, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
         } else {
             float* row = parts + r * (D + 2);
@@ -280,8 +281,8 @@ __global__ void __launch_bounds__(D) window_join_kernel(const WindowFewArgs f) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const WindowArgs& a = f.w;
-    const int r = blockIdx.x, head = blockIdx.y, b = blockIdx.z, nrep = a.q_heads / a.kv_heads, rows = a.n * nrep;
-    const float* row = f.parts + ((static_cast<long long>(b) * a.kv_heads + head) * f.splits * rows + r) * (D + 2);
+    const int r = blockIdx.x, head = blockIdx.y, b = blockIdx.z, nrep = a.q_heads / a.kv_heads, rows = f.tokens * nrep;
+    const float* row = f.parts + (((static_cast<long long>(b) * f.chunks + r / rows) * a.kv_heads + head) * f.splits * rows + r % rows) * (D + 2);
     const long long step = static_cast<long long>(rows) * (D + 2);
     float M = -INFINITY, l = 0.f, o = 0.f;
     // Eight splits at a time, all loads of them in flight together.

@@ -592,6 +592,52 @@ def test_window_repeats_bit_for_bit(gpu):
         assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
 
 
+@pytest.mark.parametrize("kin,kout", [(BF16, BF16), (F16, F32)])
+@pytest.mark.parametrize("dim,H,Hk", [(64, 2, 2), (128, 6, 2), (64, 8, 1), (128, 64, 1)])
+@pytest.mark.parametrize("n,m,window,sinks", [(65, 1024, 0, 0), (23, 1100, 1000, 4), (33, 1500, 1, 1100), (37, 2050, 0, 0)])
+def test_window_some_tokens_against_long_contexts(gpu, kin, kout, dim, H, Hk, n, m, window, sinks):
+    """More rows of a KV head than one block holds, last blocks with few of them."""
+    from ligguf_b200 import WindowConfig
+    rng = np.random.default_rng(n + m + window + H)
+    q, dq = rounded(rng.standard_normal((1, n, H, dim)), kin)
+    k, dk = rounded(rng.standard_normal((1, m, Hk, dim)), kin)
+    v, dv = rounded(rng.standard_normal((1, m, Hk, dim)), kin)
+    cfg = WindowConfig(H, Hk, dim, window, sinks, in_type=kin, out_type=kout)
+    out = run_window(cfg, dq, dk, dv, None, None, 1, n, m)
+    want = ref.window_attention(q, k, v, [m - n], [m], window, sinks, dim ** -0.5)
+    close(out, want, *window_tol(kin, kout, v))
+    assert np.array_equal(out, run_window(cfg, dq, dk, dv, None, None, 1, n, m))
+
+
+@pytest.mark.parametrize("kin", [BF16, F16])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1000, 6), (30, 1000)])
+def test_window_some_tokens_ragged_batch_and_poison(gpu, kin, window, sinks):
+    """As the ragged batch above, with blocks of one entry on both sides of its first key, its last
+    key and its window."""
+    from ligguf_b200 import WindowConfig
+    rng = np.random.default_rng(window)
+    B, n, m, H, Hk, dim = 5, 70, 1200, 4, 2, 64
+    lens = [1200, 0, 33, 1130, 1200]
+    pos0 = [1130, 0, -40, 1110, 2160]
+    q, dq = rounded(rng.standard_normal((B, n, H, dim)), kin)
+    k = rng.standard_normal((B, m, Hk, dim)).astype(np.float32)
+    v = rng.standard_normal((B, m, Hk, dim)).astype(np.float32)
+    clean, _ = rounded(v, kin)
+    for b in range(B):
+        used = set()
+        for i in range(n):
+            used |= set(ref.seen(pos0[b] + i, lens[b], window, sinks).tolist())
+        hide = [j for j in range(m) if j not in used]
+        k[b, hide], v[b, hide] = np.nan, np.inf
+    kx, dk = rounded(k, kin)
+    vx, dv = rounded(v, kin)
+    cfg = WindowConfig(H, Hk, dim, window, sinks, in_type=kin, out_type=kin)
+    out = run_window(cfg, dq, dk, dv, pos0, lens, B, n, m)
+    want = ref.window_attention(q, kx, vx, pos0, lens, window, sinks, dim ** -0.5)
+    close(out, want, *window_tol(kin, kin, clean))
+    assert not out[1].any() and not out[2, :40].any()
+
+
 def test_empty_calls_do_nothing(gpu):
     import torch
     from ligguf_b200 import QkRope, QkRopeConfig, RopeConfig, WindowAttention, WindowConfig
