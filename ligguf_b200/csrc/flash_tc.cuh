@@ -405,7 +405,7 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
 // weighted least squares (max relative error 1.03e-4, below the 2^-9 rounding of P to bf16), and
 // 2^n added into the exponent field.  x <= -127 gives 0 (x is clamped there: n = -127, f = 0);
 // -126 > x > -127 gives a value below 2^-126 that is not exact, and bf16 P then holds zero or a
-// subnormal either way.  The softmax's x never exceeds +8.
+// subnormal either way.  The softmax's x never exceeds +8 (fp16 rows: +15).
 __device__ __forceinline__ float2 exp2_poly2(float2 x) {
     x.x = fmaxf(x.x, -127.f);
     x.y = fmaxf(x.y, -127.f);
@@ -927,7 +927,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 // [64h, 64h+64) lands in columns [32h, 32h+32).  Row sum over 4 pair accumulators.
                 float2 rs4[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f),
                                  make_float2(0.f, 0.f)};
-                const float2 cc = make_float2(c2, c2), nm = make_float2(-ms, -ms);
+                // fp16 weights lie in [0, 2^15], not [0, 2^8]: the smallest then lose nothing that counts beside the
+                // row's largest (below 2^-14 a half has fewer bits; 8192 keys of weight 2^-26 would vanish).
+                const float up = kBf16 ? ms : ms - 7.f;
+                const float2 cc = make_float2(c2, c2), nm = make_float2(-up, -up);
                 {
                     uint32_t pk[32];
 #pragma unroll

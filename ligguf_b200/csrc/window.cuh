@@ -202,12 +202,14 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
                 m[u] = mx[u];
                 l[u] *= fac[u];
             }
+            // (fp16 weights in [0, 2^15], so that small ones keep their bits)
             uint32_t pa[4];
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const float e0 = exp2f(fmaf(c[n][2 * u], a.scale_log2, -ms[u])), e1 = exp2f(fmaf(c[n][2 * u + 1], a.scale_log2, -ms[u]));
+                    const float up = KvTraits<T>::kBf16 ? ms[u] : ms[u] - 15.f;
+                    const float e0 = exp2f(fmaf(c[n][2 * u], a.scale_log2, -up)), e1 = exp2f(fmaf(c[n][2 * u + 1], a.scale_log2, -up));
                     l[u] += e0 + e1;
                     pa[2 * n + u] = pack_16bit<T>(e0, e1);
                 }
