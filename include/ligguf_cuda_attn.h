@@ -427,14 +427,19 @@ typedef struct ligguf_window_cfg {
     long long q_stride, k_stride, v_stride; /* elements between rows (0 = packed) */
     long long q_batch_stride, k_batch_stride, v_batch_stride; /* between entries (0 = n or m rows) */
     int device;
+    int round_weights; /* 0 = the weights of the sum over v keep 16 bits (BF16) or 22 (F16); 1 = they may be rounded
+                          once to in_type, which is faster (see ligguf_cuda_window_attn_async) */
 } ligguf_window_cfg;
 typedef struct ligguf_window ligguf_window;
 int ligguf_cuda_window_init(const ligguf_window_cfg* cfg, ligguf_window** out);
 int ligguf_cuda_window_free(ligguf_window* h);
 /* Device pointers, rows 16-byte aligned (base and strides); out [batch][n][n_heads*head_dim], packed.
  * d_lens NULL: m keys each; d_pos0 NULL: the queries are each sequence's last (lens[b] - n + i).  batch
- * or n of 0 is a no-op.  The products' operands are in_type (so are the weights of the sum over v,
- * rounded once), accumulated in fp32.  The calls of one handle must not overlap on the GPU. */
+ * or n of 0 is a no-op.  Products are accumulated in fp32.  A weight of the sum over v enters as the sum
+ * of two in_type numbers, so that the result is fp32 arithmetic's to about 1e-5 of the largest value, rounded
+ * once to out_type.  With round_weights, more than 32 rows a KV head (n * n_heads / n_kv_heads) take weights
+ * rounded once to in_type and exponentials within 1.1e-4: errors up to 2^-8 (BF16) or 2^-11 (F16) + 1.1e-4 of
+ * the largest value, in a tenth to a quarter less time.  The calls of one handle must not overlap on the GPU. */
 int ligguf_cuda_window_attn_async(ligguf_window* h, int batch, int n, int m, const void* d_q,
                                   const void* d_k, const void* d_v, const int* d_pos0,
                                   const int* d_lens, void* d_out, void* stream);

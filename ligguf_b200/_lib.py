@@ -75,7 +75,8 @@ class WindowCfg(ctypes.Structure):
 
     _fields_ = [("n_heads", _i), ("n_kv_heads", _i), ("head_dim", _i), ("window", _i), ("sinks", _i), ("scale", _f),
                 ("in_type", _i), ("out_type", _i), ("q_stride", _ll), ("k_stride", _ll), ("v_stride", _ll),
-                ("q_batch_stride", _ll), ("k_batch_stride", _ll), ("v_batch_stride", _ll), ("device", _i)]
+                ("q_batch_stride", _ll), ("k_batch_stride", _ll), ("v_batch_stride", _ll), ("device", _i),
+                ("round_weights", _i)]
 
 
 class LigGufAttnError(RuntimeError):

@@ -61,14 +61,22 @@ struct TcArgs {
 
 // What the kernel computes: TcFull, BERT and causal prefill on bf16 copies, fp32 out; TcWindow, the
 // windowed form on the caller's rows (T fp16 or bf16, out T or fp32).
+// The matrix instructions take the softmax weights in the operands' 16 bits.  TcFull rounds them once (to bf16, as
+// its q, k and v are).  The windowed form's rows are the caller's own, so that rounding would be the largest error
+// of the call: with kTwo a weight is two numbers, P = hi + lo, which hold 16 (bf16) or 22 (fp16) bits of it, and
+// O += hi V + lo V.  lo takes the other half of P's S buffer.  Against 64 bits the 2-norm error is then that of
+// rounding the result (bf16 1.62e-3, fp16 2.0e-4; with weights rounded once 2.13e-3 and 2.7e-4), and every
+// exponential is ex2.approx, whose error is below lo's last bit, not the cubic's.  It costs half as many products
+// again and the softmax warps' second packing: 2048 queries, window 512: 40 us against 36; 8192 queries, window 4096:
+// 540 to 620 us against 430 to 490.  The caller may choose the rounding (round_weights).
 struct TcFull {
-    static constexpr bool kWindow = false;
+    static constexpr bool kWindow = false, kTwoWeights = false;
     using Operand = __nv_bfloat16;
     using Out = float;
 };
-template <typename T, typename O>
+template <typename T, typename O, bool kTwo>
 struct TcWindow {
-    static constexpr bool kWindow = true;
+    static constexpr bool kWindow = true, kTwoWeights = kTwo;
     using Operand = T;
     using Out = O;
 };
@@ -340,6 +348,13 @@ __device__ __forceinline__ uint32_t pack_16bit(float lo, float hi) {
     } else {
         return pack_bf16(lo, hi);
     }
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack_16bit(uint32_t x) {
+    if constexpr (!KvTraits<T>::kBf16)
+        return __half22float2(*reinterpret_cast<const __half2*>(&x));
+    else
+        return make_float2(__uint_as_float(x << 16), __uint_as_float(x & 0xFFFF0000u));
 }
 __device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
@@ -790,6 +805,10 @@ __global__ void __launch_bounds__(kTcThreads, 1)
 #pragma unroll
                             for (int kk = 1; kk < kTcKeys / 16; ++kk)
                                 umma_ts(o_tmem, p_tmem + kk * 8, desc_advance(vd, kk * 2048), kIdO, 1u);
+                            if constexpr (Mode::kTwoWeights)
+#pragma unroll
+                                for (int kk = 0; kk < kTcKeys / 16; ++kk)
+                                    umma_ts(o_tmem, p_tmem + kTcKeys / 2 + kk * 8, desc_advance(vd, kk * 2048), kIdO, 1u);
                             umma_commit(&pv_done[bf]);
                             umma_commit(&v_empty[s]);
                             if (j == n_kv - 1) umma_commit(&o_final[ob]);
@@ -933,11 +952,12 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 const float2 cc = make_float2(c2, c2), nm = make_float2(-up, -up);
                 {
                     uint32_t pk[32];
+                    uint32_t lo[Mode::kTwoWeights ? 32 : 1];
 #pragma unroll
                     for (int c = 0; c < 32; ++c) {
                         const int i = 2 * c;
                         float2 e = ffma2(make_float2(__uint_as_float(r[i]), __uint_as_float(r[i + 1])), cc, nm);
-                        if ((kTcPolyPairs >> (c & 7)) & 1u) {
+                        if (!Mode::kTwoWeights && ((kTcPolyPairs >> (c & 7)) & 1u)) {
                             e = exp2_poly2(e);
                         } else {
                             e.x = fast_exp2(e.x);
@@ -945,8 +965,13 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         }
                         pk[c] = pack_16bit<typename Mode::Operand>(e.x, e.y);
                         rs4[c & 3] = fadd2(rs4[c & 3], e);
+                        if constexpr (Mode::kTwoWeights) {
+                            const float2 d = ffma2(unpack_16bit<typename Mode::Operand>(pk[c]), make_float2(-1.f, -1.f), e);
+                            lo[c] = pack_16bit<typename Mode::Operand>(d.x, d.y);
+                        }
                     }
                     tmem_st32(s_tmem + half * 32, pk);  // P of columns [64h, 64h+64) into [32h, 32h+32)
+                    if constexpr (Mode::kTwoWeights) tmem_st32(s_tmem + kTcKeys / 2 + half * 32, lo);
                 }
                 const float2 rs2 = fadd2(fadd2(rs4[0], rs4[1]), fadd2(rs4[2], rs4[3]));
                 l = l * corr + (rs2.x + rs2.y);

@@ -309,7 +309,7 @@ int make_rows_tmap(CUtensorMap* m, const void* base, bool bf16, int D, int heads
     return LIGGUF_ATTN_OK;
 }
 
-template <typename T, typename Out, int D>
+template <typename T, typename Out, int D, bool kTwo>
 int launch_window_tc(const ligguf_window* h, const lg::WindowArgs& w, cudaStream_t st) {
     constexpr bool bf16 = lg::KvTraits<T>::kBf16;
     const int device = h->cfg.device;
@@ -319,7 +319,7 @@ int launch_window_tc(const ligguf_window* h, const lg::WindowArgs& w, cudaStream
         (rc = make_rows_tmap(&tk, w.k, bf16, D, w.kv_heads, w.k_stride, w.m, w.batch, w.k_batch, lg::kTcKeys)) ||
         (rc = make_rows_tmap(&tv, w.v, bf16, D, w.kv_heads, w.v_stride, w.m, w.batch, w.v_batch, lg::kTcKeys)))
         return rc;
-    auto kern = lg::flash_tc_kernel<D, lg::TcWindow<T, Out>>;
+    auto kern = lg::flash_tc_kernel<D, lg::TcWindow<T, Out, kTwo>>;
     static int resident[64] = {};
     int slots = device < 64 ? resident[device] : 0;
     if (slots == 0) {
@@ -371,7 +371,7 @@ int launch_window_tc(const ligguf_window* h, const lg::WindowArgs& w, cudaStream
 // CTAs of the few-rows form that leave partial sums: one wave of two an SM at most.
 long long few_most_items(int sms) { return 2ll * sms; }
 
-template <typename T, typename Out, int D, int kGroups>
+template <typename T, typename Out, int D, int kGroups, bool kTwo>
 int launch_window_few(const ligguf_window* h, const lg::WindowArgs& w, cudaStream_t st) {
     constexpr bool bf16 = lg::KvTraits<T>::kBf16;
     const int device = h->cfg.device;
@@ -380,7 +380,7 @@ int launch_window_few(const ligguf_window* h, const lg::WindowArgs& w, cudaStrea
     if ((rc = make_rows_tmap(&tk, w.k, bf16, D, w.kv_heads, w.k_stride, w.m, w.batch, w.k_batch, lg::kFewKeys)) ||
         (rc = make_rows_tmap(&tv, w.v, bf16, D, w.kv_heads, w.v_stride, w.m, w.batch, w.v_batch, lg::kFewKeys)))
         return rc;
-    auto kern = lg::window_few_kernel<T, Out, D, kGroups>;
+    auto kern = lg::window_few_kernel<T, Out, D, kGroups, kTwo>;
     static bool attr_done[64] = {};
     if (device >= 64 || !attr_done[device]) {
         LG_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lg::FewSmem<D>::kTotal)));
@@ -436,10 +436,11 @@ int launch_window_d(const ligguf_window* h, const lg::WindowArgs& a, cudaStream_
         few = chunks * a.batch * a.kv_heads <= h->num_sms / 4;
     }
     if (few && a.batch <= 65535 && a.kv_heads <= 65535) {
-        if (rows <= 16) return launch_window_few<T, Out, D, 1>(h, a, st);
-        return rows <= 32 ? launch_window_few<T, Out, D, 2>(h, a, st) : launch_window_few<T, Out, D, 4>(h, a, st);
+        if (rows <= 16) return launch_window_few<T, Out, D, 1, true>(h, a, st);
+        if (rows <= 32) return launch_window_few<T, Out, D, 2, true>(h, a, st);
+        return h->cfg.round_weights ? launch_window_few<T, Out, D, 4, false>(h, a, st) : launch_window_few<T, Out, D, 4, true>(h, a, st);
     }
-    return launch_window_tc<T, Out, D>(h, a, st);
+    return h->cfg.round_weights ? launch_window_tc<T, Out, D, false>(h, a, st) : launch_window_tc<T, Out, D, true>(h, a, st);
 }
 template <typename T, typename Out>
 int launch_window(const ligguf_window* h, const lg::WindowArgs& a, cudaStream_t st) {
@@ -790,6 +791,7 @@ int ligguf_cuda_window_init(const ligguf_window_cfg* cfg, ligguf_window** out) {
     if (c.window < 0 || c.sinks < 0 || c.window > kWindowMost || c.sinks > kWindowMost || (c.sinks && !c.window))
         return fail(LIGGUF_ATTN_EINVAL, "window %d with %d sinks", c.window, c.sinks);
     if (!(c.scale >= 0.f) || std::isinf(c.scale)) return fail(LIGGUF_ATTN_EINVAL, "scale %g", c.scale);
+    if (c.round_weights != 0 && c.round_weights != 1) return fail(LIGGUF_ATTN_EINVAL, "round_weights %d", c.round_weights);
     if (c.in_type != LIGGUF_KV_F16 && c.in_type != LIGGUF_KV_BF16)
         return fail(LIGGUF_ATTN_EUNSUPPORTED, "in_type %d (supported: F16, BF16)", c.in_type);
     if (c.out_type != c.in_type && c.out_type != LIGGUF_KV_F32)

@@ -89,8 +89,10 @@ __device__ __forceinline__ void mma_16bit(float (&d)[4], const uint32_t (&a)[4],
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// kGroups row groups; the other factor of the four warps is parts of a tile's keys.
-template <typename T, typename Out, int D, int kGroups>
+// kGroups row groups; the other factor of the four warps is parts of a tile's keys.  kTwo: weights as two numbers.
+// Up to 32 rows the second product is not seen (4 tokens over 16448 keys: 20 to 22 us both ways); with 33 to 64, or
+// in chunks, it takes up to a fifth (17 tokens, 32768 keys: 91.5 us against 76.7), and round_weights leaves it out.
+template <typename T, typename Out, int D, int kGroups, bool kTwo>
 __global__ void __launch_bounds__(32 * kFewWarps, 2)
     window_few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const WindowFewArgs f) {
     using Sm = FewSmem<D>;
@@ -202,8 +204,9 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
                 m[u] = mx[u];
                 l[u] *= fac[u];
             }
-            // (fp16 weights in [0, 2^15], so that small ones keep their bits)
-            uint32_t pa[4];
+            // Weights as two numbers, hi + lo (TcWindow says why).  Those of fp16 lie in [0, 2^15], so that small ones keep
+            // their bits.
+            uint32_t pa[4], pb[4];
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -212,6 +215,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
                     const float e0 = exp2f(fmaf(c[n][2 * u], a.scale_log2, -up)), e1 = exp2f(fmaf(c[n][2 * u + 1], a.scale_log2, -up));
                     l[u] += e0 + e1;
                     pa[2 * n + u] = pack_16bit<T>(e0, e1);
+                    if constexpr (kTwo) {
+                        const float2 hi = unpack_16bit<T>(pa[2 * n + u]);
+                        pb[2 * n + u] = pack_16bit<T>(e0 - hi.x, e1 - hi.y);
+                    }
                 }
             if (__any_sync(0xffffffffu, fac[0] != 1.f || fac[1] != 1.f))
 #pragma unroll
@@ -223,6 +230,10 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2)
                 ldmatrix4_trans(r, vb + (ch >> 3) * Sm::kChunk + key * 128 + (((ch & 7) ^ (key & 7)) << 4));
                 mma_16bit<T>(o[2 * j], pa, r[0], r[1]);
                 mma_16bit<T>(o[2 * j + 1], pa, r[2], r[3]);
+                if constexpr (kTwo) {
+                    mma_16bit<T>(o[2 * j], pb, r[0], r[1]);
+                    mma_16bit<T>(o[2 * j + 1], pb, r[2], r[3]);
+                }
             }
         }
         __syncthreads();

@@ -248,6 +248,7 @@ class WindowConfig:
     k_batch_stride: int = 0
     v_batch_stride: int = 0
     device: int = 0
+    round_weights: bool = False  # prompts: softmax weights rounded once to in_type, faster
 
     def to_c(self):
         return WindowCfg(**{f: getattr(self, f) for f, _ in WindowCfg._fields_})
