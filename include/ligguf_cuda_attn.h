@@ -409,8 +409,9 @@ int ligguf_cuda_kv4_load_async(ligguf_kv4* h, int layer, int seq0, int n_seqs, i
                                const void* d_k_blocks, const void* d_v_blocks, void* stream);
 int ligguf_cuda_kv4_store_async(ligguf_kv4* h, int layer, int seq0, int n_seqs, int pos0, int n,
                                 void* d_k_blocks, void* d_v_blocks, void* stream);
-/* Waits for `stream`, then: LIGGUF_ATTN_EINVAL if a decode since the last status call met a position
- * beyond n_context, LIGGUF_ATTN_ETIMEDOUT if a bounded in-kernel wait gave up, else 0. */
+/* Waits for `stream`, then, of the decodes since the last status call: LIGGUF_ATTN_ETIMEDOUT if a bounded
+ * in-kernel wait gave up (their results are not to be used; later ones are right again), else
+ * LIGGUF_ATTN_EINVAL if one met a position beyond n_context, else 0. */
 int ligguf_cuda_kv4_status(ligguf_kv4* h, void* stream);
 
 /* ---- long contexts: windowed attention over 16-bit rows ------------------------------------ */

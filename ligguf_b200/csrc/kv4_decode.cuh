@@ -59,11 +59,12 @@ struct Kv4DecodeArgs {
     float* parts;    // [blocks][2] partial results
     int* tickets;    // [n_rows * kv_heads], zero between calls
     float per_block; // 1 / blocks of the launch
-    int* err;
+    int* err;        // [kKv4ErrWords], in host memory
 };
 
-// Error word of the status call, beside the waits' codes: a decode position beyond the context.
-enum : int { KERR_POSITION = 16 };
+// The status call's words: a wait's code, and whether a row's position was beyond the context.  Each has its own,
+// or the later of the two would hide that a block gave up and left tickets behind.
+enum : int { kKv4ErrWait = 0, kKv4ErrPosition = 1, kKv4ErrWords = 2 };
 
 // Eight warps a block; two blocks an SM, or one of twice the registers for eight heads a KV head.  (One block of
 // sixteen warps is slower: nothing covers its starts and joins. 24 sequences: 58.8 us against 47.)
@@ -667,7 +668,7 @@ __global__ void __launch_bounds__(32 * kv4_warps(NREP), kv4_blocks_per_sm(NREP))
         for (int r = bx; r < a.n_rows; r += gridDim.x) {
             const int pos = where.at(a, r);
             if (pos >= 0 && pos < a.n_context) continue;
-            if (pos >= 0 && threadIdx.x == 0) *reinterpret_cast<volatile int*>(a.err) = KERR_POSITION;
+            if (pos >= 0 && threadIdx.x == 0) reinterpret_cast<volatile int*>(a.err)[kKv4ErrPosition] = 1;
             const float z[8] = {};
             for (int u = threadIdx.x; u < a.q_heads * L; u += kThreads)
                 store8(static_cast<In*>(a.out) + (static_cast<long long>(r) * a.q_heads * L + u) * 8, z);
@@ -816,7 +817,7 @@ __global__ void __launch_bounds__(32 * kv4_warps(NREP), kv4_blocks_per_sm(NREP))
             if (!mbar_try_wait(&bars[s], (taken / S) & 1) && !mbar_wait_bounded(&bars[s], (taken / S) & 1, deadline, abort)) {
                 // (the tile is worked on as it is; the block stops at the next barrier)
                 *abort = 1;
-                *reinterpret_cast<volatile int*>(a.err) = KERR_TIMEOUT_FULL;
+                reinterpret_cast<volatile int*>(a.err)[kKv4ErrWait] = KERR_TIMEOUT_FULL;
             }
             const int k0 = kv4_tile_of(at.r, at.t) * kKv4Tile;
             const int k1 = at.t + 1 == at.r.ns ? at.r.tw * kKv4Tile : k0 + kKv4Tile;

@@ -155,10 +155,10 @@ int launch_rope_rows_any(lg::RopeRowsArgs& a, const ligguf_rope_cfg& r, int in_t
     }
 }
 
-int make_err_word(int** h_err, int** d_err) {
+int make_err_words(int** h_err, int** d_err) {
     if (cudaHostAlloc(reinterpret_cast<void**>(h_err), 64, cudaHostAllocMapped) != cudaSuccess)
-        return fail(LIGGUF_ATTN_ENOMEM, "mapped error word");
-    **h_err = 0;
+        return fail(LIGGUF_ATTN_ENOMEM, "mapped error words");
+    std::memset(*h_err, 0, 64);
     LG_CUDA(cudaHostGetDevicePointer(reinterpret_cast<void**>(d_err), *h_err, 0));
     return LIGGUF_ATTN_OK;
 }
@@ -603,7 +603,7 @@ int ligguf_cuda_kv4_init(const ligguf_kv4_cfg* cfg, ligguf_kv4** out) {
     if (cudaMemset(h->tickets, 0, ticket_bytes) != cudaSuccess) return bail(fail(LIGGUF_ATTN_ECUDA, "cudaMemset of the tickets failed"));
     // Zeroed like the engine's cache: unwritten positions are zeros, not whatever lay there.
     if (cudaMemset(h->tiles, 0, bytes) != cudaSuccess) return bail(fail(LIGGUF_ATTN_ECUDA, "cudaMemset of the cache failed"));
-    if ((rc = make_turns(c.rope, &h->turns)) || (rc = make_err_word(&h->h_err, &h->d_err))) return bail(rc);
+    if ((rc = make_turns(c.rope, &h->turns)) || (rc = make_err_words(&h->h_err, &h->d_err))) return bail(rc);
     *out = h;
     return LIGGUF_ATTN_OK;
 }
@@ -760,13 +760,15 @@ int ligguf_cuda_kv4_status(ligguf_kv4* h, void* stream) {
     if (!h) return fail(LIGGUF_ATTN_EINVAL, "null handle");
     DeviceGuard dg(h->cfg.device);
     LG_CUDA(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
-    const int code = *reinterpret_cast<volatile int*>(h->h_err);
-    *reinterpret_cast<volatile int*>(h->h_err) = 0;
-    if (code == lg::KERR_POSITION) return fail(LIGGUF_ATTN_EINVAL, "a decode row's position is beyond n_context %d", h->cfg.n_context);
+    volatile int* words = h->h_err;
+    const int code = words[lg::kKv4ErrWait], beyond = words[lg::kKv4ErrPosition];
+    words[lg::kKv4ErrWait] = words[lg::kKv4ErrPosition] = 0;
     if (code) {  // blocks that gave up left tickets behind
         LG_CUDA(cudaMemset(h->tickets, 0, size_t(h->cfg.n_seqs) * h->cfg.n_kv_heads * sizeof(int)));
-        return fail(LIGGUF_ATTN_ETIMEDOUT, "a bounded in-kernel wait gave up (kernel error code %d)", code);
+        return fail(LIGGUF_ATTN_ETIMEDOUT, "a bounded in-kernel wait gave up (kernel error code %d)%s", code,
+                    beyond ? "; a decode row's position was beyond n_context too" : "");
     }
+    if (beyond) return fail(LIGGUF_ATTN_EINVAL, "a decode row's position is beyond n_context %d", h->cfg.n_context);
     return LIGGUF_ATTN_OK;
 }
 
@@ -818,7 +820,7 @@ int ligguf_cuda_window_init(const ligguf_window_cfg* cfg, ligguf_window** out) {
         (void)cudaGetLastError();
         return bail(fail(LIGGUF_ATTN_ENOMEM, "handle buffers"));
     }
-    if ((rc = make_err_word(&h->h_err, &h->d_err))) return bail(rc);
+    if ((rc = make_err_words(&h->h_err, &h->d_err))) return bail(rc);
     *out = h;
     return LIGGUF_ATTN_OK;
 }
