@@ -503,6 +503,16 @@ __device__ __forceinline__ bool tc_window_fix(const TcArgs& a, const TcWinItem& 
     return k0 + kTcKeys > it.hi || (k0 < it.lo && k0 + kTcKeys > a.sinks);
 }
 static_assert(sizeof(TcWinItem) == kTcItemInts * 4, "the items' room in shared memory");
+// Windowed: tiles whose V warp 3 is asked about, those to be zeroed and every item's first, which has it keep pace
+// with the products.
+__device__ __forceinline__ bool tc_window_ask(bool fix, int j) { return fix || j == 0; }
+// How long a role may wait within an item.  A windowed item may have two million key tiles, so its limit grows with
+// them (about 1.4 us a tile; ten times that).
+constexpr uint64_t kTcTileNs = 14000;
+template <typename Mode>
+__device__ __forceinline__ uint64_t tc_deadline(int tiles) {
+    return globaltimer_ns() + kWaitLimitNs + (Mode::kWindow ? uint64_t(tiles) * kTcTileNs : 0);
+}
 template <typename Mode>
 __device__ __forceinline__ auto tc_any_item(const TcArgs& a, const void* items, int w, int idx, int n_qt) {
     if constexpr (Mode::kWindow)
@@ -556,8 +566,8 @@ __global__ void __launch_bounds__(kTcThreads, 1)
     uint64_t* o_free = o_final + 2;   // [2] the epilogue has read O
     uint64_t* l_full = o_free + 2;
     uint64_t* xchg = l_full + LR;     // [tile parity][quarter] both halves of the rows wrote their maxima    // [LR] the item's row sums are in shared memory
-    // Windowed: the P.V issuer asks for an edge tile's unseen rows of V to be zeroed, and they are.  One tile
-    // at a time, so both barriers advance a phase per edge tile.
+    // Windowed: the P.V issuer asks for a tile's unseen rows of V to be zeroed, and they are.  One tile at a time,
+    // so both barriers advance a phase per tile asked about (tc_window_ask).
     uint64_t* v_ask = xchg + 8;
     uint64_t* v_fixed = v_ask + 1;
     float* lsum = reinterpret_cast<float*>(sm + Sm::kL);
@@ -630,7 +640,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     if (idx < 0) break;
                     const auto it = tc_any_item<Mode>(a, items, w, idx, n_qt);
                     if (it.n_kv == 0) continue;
-                    deadline = globaltimer_ns() + kWaitLimitNs;
+                    deadline = tc_deadline<Mode>(it.n_kv);
                     // Q of item z into buffer z & 1, once the last S MMA of item z - 2 has read it.
                     const int qb = z & 1;
                     if (z >= 2 &&
@@ -697,17 +707,26 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if constexpr (kWin) {
                 bool ok = true;
                 int t = 0, asked = 0;
+                int since = 0;  // tiles since the last that it was asked about: its limit runs from there
                 for (int w = 0; ok; ++w) {
                     const int idx = tc_walk(a, w, n_items);
                     if (idx < 0) break;
                     const auto it = tc_any_item<Mode>(a, items, w, idx, n_qt);
-                    const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
                     for (int j = 0; j < it.n_kv; ++j, ++t) {
                         const int s = t % S, k0 = tc_window_key0(it, j);
-                        if (!tc_window_fix(a, it, k0)) continue;
+                        const bool fix = tc_window_fix(a, it, k0);
+                        ++since;
+                        if (!tc_window_ask(fix, j)) continue;
+                        const uint64_t deadline = tc_deadline<Mode>(since);
                         ok = __all_sync(0xffffffffu, tc_wait(v_ask, asked & 1, deadline, abort, a.err, KERR_TIMEOUT_FULL));
                         if (!ok) break;
                         ++asked;
+                        since = 0;
+                        if (!fix) {
+                            __syncwarp();
+                            if (lane == 0) mbar_arrive(v_fixed);
+                            continue;
+                        }
                         // Eight lanes a 128-byte row (a lane a row would put all 32 on the same banks: 1.1 us an item).
                         for (int r = lane >> 3; r < kTcKeys; r += 4) {
                             const int key = k0 + r;
@@ -741,14 +760,14 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                 bool ok = true;
                 uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
                 int t = 0, z = 0;
-                int asked = 0;  // edge tiles so far
+                int asked = 0;  // tiles that warp 3 was asked about so far
                 for (int w = 0; ok; ++w) {
                     const int idx = tc_walk(a, w, n_items);
                     if (idx < 0) break;
                     const auto it = tc_any_item<Mode>(a, items, w, idx, n_qt);
                     const int n_kv = it.n_kv;
                     if (n_kv == 0) continue;
-                    deadline = globaltimer_ns() + kWaitLimitNs;
+                    deadline = tc_deadline<Mode>(n_kv);
                     const int qb = z & 1, ob = z & 1;
                     if (is_s) {
                         if (!tc_wait(&q_full[qb], (z >> 1) & 1, deadline, abort, a.err, KERR_TIMEOUT_FULL)) break;
@@ -777,9 +796,9 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                     } else {
                         for (int j = 0; j < n_kv; ++j, ++t) {
                             const int s = t % S, bf = t & 1;
-                            bool fix = false;
-                            if constexpr (kWin) fix = tc_window_fix(a, it, tc_window_key0(it, j));
-                            if (fix) {  // warp 3 zeroes V's unseen rows while the softmax works on the tile
+                            bool ask = false;
+                            if constexpr (kWin) ask = tc_window_ask(tc_window_fix(a, it, tc_window_key0(it, j)), j);
+                            if (ask) {  // warp 3 zeroes V's unseen rows while the softmax works on the tile
                                 if (!tc_wait(&v_full[s], (t / S) & 1, deadline, abort, a.err, KERR_TIMEOUT_FULL)) {
                                     ok = false;
                                     break;
@@ -792,11 +811,11 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                                  !tc_wait(&o_free[ob], ((z >> 1) - 1) & 1, deadline, abort, a.err, KERR_TIMEOUT_MMA)) ||
                                 !tc_wait(&p_full[bf], (t >> 1) & 1, deadline, abort, a.err, KERR_TIMEOUT_MMA) ||
                                 !tc_wait(&v_full[s], (t / S) & 1, deadline, abort, a.err, KERR_TIMEOUT_FULL) ||
-                                (fix && !tc_wait(v_fixed, asked & 1, deadline, abort, a.err, KERR_TIMEOUT_FULL))) {
+                                (ask && !tc_wait(v_fixed, asked & 1, deadline, abort, a.err, KERR_TIMEOUT_FULL))) {
                                 ok = false;
                                 break;
                             }
-                            if (fix) ++asked;
+                            if (ask) ++asked;
                             tc_fence_after();
                             const uint32_t p_tmem = tmem + Tm::kS + bf * kTcKeys;  // P(t) packed in its S buffer
                             const uint32_t o_tmem = tmem + Tm::kO + ob * D;
@@ -847,7 +866,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
             if (idx < 0) break;
             const auto it = tc_any_item<Mode>(a, items, w, idx, n_qt);
             if (it.n_kv == 0) continue;
-            const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
+            const uint64_t deadline = tc_deadline<Mode>(it.n_kv);
             const int qr = it.r0 + row;  // query row within the sequence
             const int r0 = it.r0, kv_len = it.kv_len, n_kv = it.n_kv;
             int win_p0 = 0;  // position of the tile's first row
@@ -1022,7 +1041,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
                         tc_store4(obase + rr * ostride + 4 * (lane % F4), make_float4(0.f, 0.f, 0.f, 0.f));
                 continue;
             }
-            const uint64_t deadline = globaltimer_ns() + kWaitLimitNs;
+            const uint64_t deadline = tc_deadline<Mode>(it.n_kv);
             const int ob = z & 1;
             ok = __all_sync(0xffffffffu, tc_wait(&l_full[z % LR], (z / LR) & 1, deadline, abort, a.err,
                                                  KERR_TIMEOUT_MMA));

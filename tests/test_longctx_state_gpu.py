@@ -59,3 +59,35 @@ def test_kv4_decode_recovers_from_a_wait_that_gave_up(gpu, position_too):
         want = decode_ref(c, kb, vb, qkv, pos)
         close(out, want, 2e-5 * np.abs(want).max())
     c.status()
+
+
+def test_window_entries_after_more_than_two_seconds_of_work(gpu):
+    """Entry 0: 2^19 tokens without a window, so that none of its key tiles has rows to be hidden, about three seconds
+    of work; entry 1: 200 keys, with such rows.  The kernel's waits are bounded to two seconds each, and none of them
+    may count the time before its own item.  Rows of both entries against 64 bits; bound: see
+    test_longctx_accuracy_gpu.py (equal values keep entry 0's sums, of half a million keys, apart from the cut)."""
+    import torch
+    from ligguf_b200 import WindowAttention, WindowConfig
+    g = torch.Generator(device="cuda").manual_seed(5)
+    B, n, H, dim, short = 2, 1 << 19, 48, 64, 200
+    q = torch.randn(B, n, H * dim, generator=g, device="cuda", dtype=torch.bfloat16)
+    k, v = (torch.randn(B, n, dim, generator=g, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    v[0] = v[0, 0]
+    out = torch.full_like(q, float("nan"))
+    h = WindowAttention(WindowConfig(H, 1, dim))
+    begin, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    begin.record()
+    h.attn_async(B, n, n, q, k, v, out, d_pos0=torch.zeros(2, dtype=torch.int32, device="cuda"),
+                 d_lens=torch.tensor([n, short], dtype=torch.int32, device="cuda"))
+    end.record()
+    h.status()
+    assert begin.elapsed_time(end) > 2100, "too little work for what this test is about"
+    assert not torch.isnan(out).any()
+    for b, rows in ((0, (0, 1, 127, 128, 4000)), (1, (0, 63, 127, 128, 199, 200, 5000, n - 1))):
+        for i in rows:
+            seen = min(i + 1, n if b == 0 else short)
+            s = q[b, i].double().view(H, dim) @ k[b, :seen].double().T * dim ** -0.5
+            want = torch.softmax(s, -1) @ v[b, :seen].double()
+            close(out[b, i].double().view(H, dim).cpu().numpy(), want.cpu().numpy(), 5e-5 * float(v[b].abs().max()), 2.0 ** -8)
+    last = out[0, -1].double().view(H, dim).cpu().numpy()
+    close(last, np.broadcast_to(v[0, 0].double().cpu().numpy(), last.shape), 0.0, 2.0 ** -8 + 2.0 ** -8)
