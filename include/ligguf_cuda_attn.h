@@ -378,7 +378,8 @@ typedef struct ligguf_kv4_cfg {
 typedef struct ligguf_kv4 ligguf_kv4;
 int ligguf_cuda_kv4_init(const ligguf_kv4_cfg* cfg, ligguf_kv4** out);
 int ligguf_cuda_kv4_free(ligguf_kv4* h);
-/* One layer's norm weights, head_dim floats each (host), before its first append or decode with qk_norm. */
+/* One layer's norm weights, head_dim floats each (host), before its first append or decode with qk_norm.  They are
+ * in place when the call returns; calls that use them must not be running. */
 int ligguf_cuda_kv4_set_qk_norm(ligguf_kv4* h, int layer, const float* q_gamma, const float* k_gamma);
 /* A prompt's n tokens (0 is a no-op) at positions [pos0, pos0 + n) of sequence seq: norms and rotates q
  * and k, quantizes k and v into the cache, and writes, where the pointer is not NULL, the queries

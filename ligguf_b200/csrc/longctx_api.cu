@@ -71,6 +71,13 @@ int check_rope(const ligguf_rope_cfg& r) {
     return LIGGUF_ATTN_OK;
 }
 
+// Waits for what the set-up calls put on the legacy stream (copies from pageable memory, which return when they are
+// staged, and memsets): the callers' streams may be non-blocking ones, which do not wait for that stream.
+int set_up_done() {
+    LG_CUDA(cudaStreamSynchronize(cudaStreamLegacy));
+    return LIGGUF_ATTN_OK;
+}
+
 // Turns per position of every pair, in device memory.
 int make_turns(const ligguf_rope_cfg& r, double** out) {
     double t[64];
@@ -94,7 +101,7 @@ int make_turns(const ligguf_rope_cfg& r, double** out) {
     if (cudaMalloc(reinterpret_cast<void**>(out), sizeof(t)) != cudaSuccess)
         return fail(LIGGUF_ATTN_ENOMEM, "rotation table");
     LG_CUDA(cudaMemcpy(*out, t, pairs * sizeof(double), cudaMemcpyHostToDevice));
-    return LIGGUF_ATTN_OK;
+    return set_up_done();
 }
 
 int rope_layout(const ligguf_rope_cfg& r) {
@@ -603,7 +610,7 @@ int ligguf_cuda_kv4_init(const ligguf_kv4_cfg* cfg, ligguf_kv4** out) {
     if (cudaMemset(h->tickets, 0, ticket_bytes) != cudaSuccess) return bail(fail(LIGGUF_ATTN_ECUDA, "cudaMemset of the tickets failed"));
     // Zeroed like the engine's cache: unwritten positions are zeros, not whatever lay there.
     if (cudaMemset(h->tiles, 0, bytes) != cudaSuccess) return bail(fail(LIGGUF_ATTN_ECUDA, "cudaMemset of the cache failed"));
-    if ((rc = make_turns(c.rope, &h->turns)) || (rc = make_err_words(&h->h_err, &h->d_err))) return bail(rc);
+    if ((rc = make_turns(c.rope, &h->turns)) || (rc = make_err_words(&h->h_err, &h->d_err)) || (rc = set_up_done())) return bail(rc);
     *out = h;
     return LIGGUF_ATTN_OK;
 }
@@ -616,6 +623,7 @@ int ligguf_cuda_kv4_set_qk_norm(ligguf_kv4* h, int layer, const float* q_gamma, 
     float* g = h->gammas + size_t(layer) * 2 * D;
     LG_CUDA(cudaMemcpy(g, q_gamma, D * sizeof(float), cudaMemcpyHostToDevice));
     LG_CUDA(cudaMemcpy(g + D, k_gamma, D * sizeof(float), cudaMemcpyHostToDevice));
+    if (const int rc = set_up_done()) return rc;
     h->norm_set[layer] = 1;
     return LIGGUF_ATTN_OK;
 }
@@ -764,7 +772,9 @@ int ligguf_cuda_kv4_status(ligguf_kv4* h, void* stream) {
     const int code = words[lg::kKv4ErrWait], beyond = words[lg::kKv4ErrPosition];
     words[lg::kKv4ErrWait] = words[lg::kKv4ErrPosition] = 0;
     if (code) {  // blocks that gave up left tickets behind
-        LG_CUDA(cudaMemset(h->tickets, 0, size_t(h->cfg.n_seqs) * h->cfg.n_kv_heads * sizeof(int)));
+        const cudaStream_t st = static_cast<cudaStream_t>(stream);
+        LG_CUDA(cudaMemsetAsync(h->tickets, 0, size_t(h->cfg.n_seqs) * h->cfg.n_kv_heads * sizeof(int), st));
+        LG_CUDA(cudaStreamSynchronize(st));
         return fail(LIGGUF_ATTN_ETIMEDOUT, "a bounded in-kernel wait gave up (kernel error code %d)%s", code,
                     beyond ? "; a decode row's position was beyond n_context too" : "");
     }

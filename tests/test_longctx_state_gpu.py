@@ -91,3 +91,33 @@ def test_window_entries_after_more_than_two_seconds_of_work(gpu):
             close(out[b, i].double().view(H, dim).cpu().numpy(), want.cpu().numpy(), 5e-5 * float(v[b].abs().max()), 2.0 ** -8)
     last = out[0, -1].double().view(H, dim).cpu().numpy()
     close(last, np.broadcast_to(v[0, 0].double().cpu().numpy(), last.shape), 0.0, 2.0 ** -8 + 2.0 ** -8)
+
+
+@pytest.mark.parametrize("rope_dim", [0, 128])
+def test_kv4_cache_is_ready_for_any_stream(gpu, rope_dim):
+    """A cache of 9.7 GB, whose zeroing takes the GPU some milliseconds, then at once a load on a stream that does not
+    wait for the legacy stream: what was loaded stays, the rest is zeros.  The norm weights are there as well."""
+    import torch
+    import longctx_ref as ref
+    n, Hk, last = 1 << 20, 8, 7
+    kb, vb = (torch.randint(0, 256, (1, 64, Hk * 4, 18), dtype=torch.uint8, device="cuda") for _ in range(2))
+    q, k, v = (torch.randn(1, w, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda") for w in (1024,) * 3)
+    got = [torch.full_like(kb, 7) for _ in range(2)]
+    rows = [torch.full((1, 1024), float("nan"), device="cuda") for _ in range(3)]
+    before = [torch.full_like(kb, 7) for _ in range(2)]
+    g = (1 + 0.1 * np.random.default_rng(3).standard_normal((2, 128))).astype(np.float32)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    c = make_cache(128, Hk, 1, n_context=n, n_layers=last + 1, rope_dim=rope_dim, qk_norm=True, rows_type=F32)
+    with torch.cuda.stream(side):
+        c.load_async(last, 0, 1, n - 64, 64, kb, vb)
+        c.set_qk_norm(last, g[0], g[1])
+        c.append_async(last, 0, 0, 1, q, k, v, rows[0], rows[1], rows[2])
+        c.store_async(last, 0, 1, n - 64, 64, *got)
+        c.store_async(last, 0, 1, n - 128, 64, *before)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], kb) and torch.equal(got[1], vb)
+    assert not any(x.any() for x in before)
+    want = ref.rms(q.cpu().numpy().reshape(1, 8, 128), g[0], 1e-6)  # (position 0: no rotation)
+    close(rows[0].cpu().numpy().reshape(1, 8, 128), want, 1e-5 * np.abs(want).max())
+    c.status(stream=side)
