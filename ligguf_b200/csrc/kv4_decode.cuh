@@ -193,7 +193,7 @@ __device__ __forceinline__ void kv4_head(float (&x)[8], const float* gamma, bool
 #pragma unroll
         for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
         ss = head_sum<L>(ss);
-        const float rs = 1.0f / sqrtf(ss / static_cast<float>(D) + eps);
+        const float rs = rms_factor<D>(ss, eps);
         float gm[8];
         load8(gamma + l * 8, gm);
 #pragma unroll
@@ -205,8 +205,8 @@ __device__ __forceinline__ void kv4_head(float (&x)[8], const float* gamma, bool
             if (4 * l + i < pairs) {
                 const float2 w = cs[4 * l + i];
                 const float x0 = x[2 * i], x1 = x[2 * i + 1];
-                x[2 * i] = x0 * w.x - x1 * w.y;
-                x[2 * i + 1] = x0 * w.y + x1 * w.x;
+                x[2 * i] = rope_first(x0, x1, w);
+                x[2 * i + 1] = rope_second(x0, x1, w);
             }
     } else if (pairs) {
         if (lane < L) store8(dst + l * 8, x);
@@ -218,7 +218,7 @@ __device__ __forceinline__ void kv4_head(float (&x)[8], const float* gamma, bool
                 const bool low = e < pairs;
                 const float2 w = cs[low ? e : e - pairs];
                 const float other = dst[low ? e + pairs : e - pairs];
-                x[i] = x[i] * w.x + (low ? -other : other) * w.y;
+                x[i] = low ? rope_first(x[i], other, w) : rope_second(other, x[i], w);
             }
         }
         __syncwarp();

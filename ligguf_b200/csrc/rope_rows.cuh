@@ -51,6 +51,18 @@ __device__ __forceinline__ float head_sum(float v) {
     return v;
 }
 
+// What a head's elements are multiplied by, from the sum of their squares.  (One rounding: 1 / sqrtf has two, a 2-norm
+// error of 8.5e-8 in place of 7.5e-8, and takes the prompts' kernel from 33 to 41.7 us for 7777 tokens.)
+template <int D>
+__device__ __forceinline__ float rms_factor(float ss, float eps) {
+    return rsqrtf(fmaf(ss, 1.0f / D, eps));
+}
+// The rotation of a pair (a, b) by w = (cos, sin), with its roundings spelt out: both kernels that write the cache take
+// these and rms_factor, so that a key is the same there whether it came with a prompt or alone.  (rope_pairs_kernel,
+// which writes none, leaves the roundings to the compiler: 32.8 us for its prompt, 38.7 with these.)
+__device__ __forceinline__ float rope_first(float a, float b, float2 w) { return fmaf(a, w.x, -__fmul_rn(b, w.y)); }
+__device__ __forceinline__ float rope_second(float a, float b, float2 w) { return fmaf(b, w.x, __fmul_rn(a, w.y)); }
+
 // Layouts of the rotation: adjacent pairs lie within a thread; halves whose distance is a whole number
 // of units are exchanged by a shuffle, others through shared memory.
 enum : int { kRopeAdjacent = 0, kRopeHalves = 1, kRopeHalvesOdd = 2 };
@@ -94,7 +106,7 @@ __device__ __forceinline__ void rope_rows_unit(const RopeRowsArgs& a, long long 
         for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
         ss = head_sum<L>(ss);
         if (kind < 2) {
-            const float rs = rsqrtf(ss * (1.0f / D) + a.eps);
+            const float rs = rms_factor<D>(ss, a.eps);
             float g[8];
             load8((kind ? a.k_gamma : a.q_gamma) + l * 8, g);
 #pragma unroll
@@ -108,8 +120,8 @@ __device__ __forceinline__ void rope_rows_unit(const RopeRowsArgs& a, long long 
                 if (4 * l + i < a.pairs) {
                     const float2 w = cs[rope_slot<kLayout>(4 * l + i)];
                     const float x0 = x[2 * i], x1 = x[2 * i + 1];
-                    x[2 * i] = x0 * w.x - x1 * w.y;
-                    x[2 * i + 1] = x0 * w.y + x1 * w.x;
+                    x[2 * i] = rope_first(x0, x1, w);
+                    x[2 * i + 1] = rope_second(x0, x1, w);
                 }
     } else if constexpr (kLayout == kRopeHalves) {
         const int hl = a.pairs / 8;  // units of a half
@@ -120,7 +132,7 @@ __device__ __forceinline__ void rope_rows_unit(const RopeRowsArgs& a, long long 
             const float other = __shfl_sync(0xffffffffu, x[i], from & (L - 1), L);
             if (kind < 2 && l < 2 * hl) {
                 const float2 w = cs[rope_slot<kLayout>(8 * (low ? l : l - hl) + i)];
-                x[i] = x[i] * w.x + (low ? -other : other) * w.y;
+                x[i] = low ? rope_first(x[i], other, w) : rope_second(other, x[i], w);
             }
         }
     } else {
@@ -138,7 +150,7 @@ __device__ __forceinline__ void rope_rows_unit(const RopeRowsArgs& a, long long 
                     const bool low = e < a.pairs;
                     const float2 w = cs[rope_slot<kLayout>(low ? e : e - a.pairs)];
                     const float other = hx[low ? e + a.pairs : e - a.pairs];
-                    x[i] = x[i] * w.x + (low ? -other : other) * w.y;
+                    x[i] = low ? rope_first(x[i], other, w) : rope_second(other, x[i], w);
                 }
             }
     }
@@ -244,7 +256,7 @@ __global__ void __launch_bounds__(256, 4) rope_pairs_kernel(const RopeRowsArgs a
 #pragma unroll
             for (int n = 0; n < kTake; ++n) rs[n] += __shfl_xor_sync(0xffffffffu, rs[n], o);
 #pragma unroll
-        for (int n = 0; n < kTake; ++n) rs[n] = rsqrtf(rs[n] * (1.0f / D) + a.eps);
+        for (int n = 0; n < kTake; ++n) rs[n] = rms_factor<D>(rs[n], a.eps);
     }
     float4 w[4];  // two rotations each
 #pragma unroll

@@ -10,7 +10,8 @@ import numpy as np
 import pytest
 
 import longctx_ref as ref
-from test_longctx_gpu import BF16, F16, F32, HALF_ULP, close, dev, host, rounded, run_window, window_tol
+from test_longctx_gpu import (BF16, F16, F32, HALF_ULP, close, dev, make_cache, rounded, run_window, store,
+                              window_tol)
 
 pytestmark = pytest.mark.gpu
 
@@ -69,3 +70,26 @@ def test_window_many_small_weights_add_up(gpu, kin, n, round_weights):
     small = np.exp(-18.0) * (m - n + np.arange(n))
     want = np.broadcast_to((small / (1 + small))[None, :, None, None], out.shape)
     close(out, want, 0, 2.0 ** -5)
+
+
+@pytest.mark.parametrize("kin", [F32, F16, BF16])
+@pytest.mark.parametrize("dim,rope_dim,layout", [(128, 128, "adjacent"), (128, 128, "halves"), (64, 64, "halves"),
+                                                 (128, 96, "halves"), (64, 20, "halves"), (64, 0, "adjacent")])
+def test_token_is_held_alike_whichever_call_brought_it(gpu, kin, dim, rope_dim, layout):
+    """A token's key and value are the same in the cache, bit for bit, whether append or decode wrote them."""
+    import torch
+    rng = np.random.default_rng(dim + rope_dim)
+    n, Hk, nrep, pos0 = 300, 3, 2, 1000
+    kw = dict(n_context=pos0 + n, rope_dim=rope_dim, layout=layout, qk_norm=True, in_type=kin, rows_type=F32)
+    g = (1 + 0.1 * rng.standard_normal((2, dim))).astype(np.float32)
+    a, b = make_cache(dim, Hk, nrep, **kw), make_cache(dim, Hk, nrep, n_seqs=n, **kw)
+    a.set_qk_norm(0, g[0], g[1])
+    b.set_qk_norm(0, g[0], g[1])
+    q, k, v = (rounded(rng.standard_normal((n, h * dim)) * 2, kin)[1] for h in (Hk * nrep, Hk, Hk))
+    a.append_async(0, 0, pos0, n, None, k, v)
+    out = torch.empty_like(q)
+    b.decode_async(0, n, q, k, v, out, d_pos=torch.arange(pos0, pos0 + n, dtype=torch.int32, device="cuda"))
+    ka, va = store(a, 0, 0, 1, pos0, n)
+    kb, vb = store(b, 0, 0, n, pos0, n)
+    each = np.arange(n)
+    assert np.array_equal(va[0], vb[each, each]) and np.array_equal(ka[0], kb[each, each])
