@@ -67,12 +67,9 @@ __device__ __forceinline__ float rope_second(float a, float b, float2 w) { retur
 // of units are exchanged by a shuffle, others through shared memory.
 enum : int { kRopeAdjacent = 0, kRopeHalves = 1, kRopeHalvesOdd = 2 };
 
-// The table of a token's rotations: pair i's cosine and sine.
-template <int kLayout>
-__device__ __forceinline__ int rope_slot(int i) {
-    // Threads of neighbouring units read neighbouring entries (an entry of two pairs, read as 16 bytes).
-    return kLayout == kRopeHalves ? ((i & 7) >> 1) * 16 + (i >> 3) * 2 + (i & 1) : (i & 1) + ((i >> 1) & 3) * 16 + (i >> 3) * 2;
-}
+// The place of pair i's cosine and sine in a token's table: threads of neighbouring units read neighbouring entries
+// (an entry of two pairs, read as 16 bytes).
+__device__ __forceinline__ int rope_slot(int i) { return ((i & 7) >> 1) * 16 + (i >> 3) * 2 + (i & 1); }
 
 // 8 elements of a row as they were loaded.
 template <typename T>
@@ -118,7 +115,7 @@ __device__ __forceinline__ void rope_rows_unit(const RopeRowsArgs& a, long long 
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 if (4 * l + i < a.pairs) {
-                    const float2 w = cs[rope_slot<kLayout>(4 * l + i)];
+                    const float2 w = cs[rope_slot(4 * l + i)];
                     const float x0 = x[2 * i], x1 = x[2 * i + 1];
                     x[2 * i] = rope_first(x0, x1, w);
                     x[2 * i + 1] = rope_second(x0, x1, w);
@@ -131,7 +128,7 @@ __device__ __forceinline__ void rope_rows_unit(const RopeRowsArgs& a, long long 
         for (int i = 0; i < 8; ++i) {
             const float other = __shfl_sync(0xffffffffu, x[i], from & (L - 1), L);
             if (kind < 2 && l < 2 * hl) {
-                const float2 w = cs[rope_slot<kLayout>(8 * (low ? l : l - hl) + i)];
+                const float2 w = cs[rope_slot(8 * (low ? l : l - hl) + i)];
                 x[i] = low ? rope_first(x[i], other, w) : rope_second(other, x[i], w);
             }
         }
@@ -148,7 +145,7 @@ __device__ __forceinline__ void rope_rows_unit(const RopeRowsArgs& a, long long 
                 const int e = 8 * l + i;
                 if (e < 2 * a.pairs) {
                     const bool low = e < a.pairs;
-                    const float2 w = cs[rope_slot<kLayout>(low ? e : e - a.pairs)];
+                    const float2 w = cs[rope_slot(low ? e : e - a.pairs)];
                     const float other = hx[low ? e + a.pairs : e - a.pairs];
                     x[i] = low ? rope_first(x[i], other, w) : rope_second(other, x[i], w);
                 }
@@ -205,7 +202,7 @@ __global__ void __launch_bounds__(256, 4) rope_pairs_kernel(const RopeRowsArgs a
     const int item = blockIdx.x % a.parts * blockDim.x + threadIdx.x;
     auto table = [&]() {
         if (threadIdx.x < 64)
-            cs[rope_slot<kLayout>(threadIdx.x)] = static_cast<int>(threadIdx.x) < a.pairs ? rope_turn(a.turns[threadIdx.x], pos, a.magnitude) : make_float2(1.f, 0.f);
+            cs[rope_slot(threadIdx.x)] = static_cast<int>(threadIdx.x) < a.pairs ? rope_turn(a.turns[threadIdx.x], pos, a.magnitude) : make_float2(1.f, 0.f);
         __syncthreads();
     };  // (whole warps: pair_items is a multiple of 32)
     const int qh = a.q ? a.q_heads : 0, heads = qh + a.kv_heads;
@@ -261,7 +258,7 @@ __global__ void __launch_bounds__(256, 4) rope_pairs_kernel(const RopeRowsArgs a
     float4 w[4];  // two rotations each
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        w[i] = kLayout == kRopeAdjacent || dl < a.pairs / 8 ? *reinterpret_cast<const float4*>(cs + rope_slot<kLayout>(8 * dl + 2 * i))
+        w[i] = kLayout == kRopeAdjacent || dl < a.pairs / 8 ? *reinterpret_cast<const float4*>(cs + rope_slot(8 * dl + 2 * i))
                                                             : make_float4(1.f, 0.f, 1.f, 0.f);
     Out* dst = keys ? static_cast<Out*>(a.k_out) + tok * a.k_out_stride - qh * D : static_cast<Out*>(a.q_out) + tok * a.q_out_stride;
 #pragma unroll
@@ -305,7 +302,7 @@ __global__ void __launch_bounds__(256) rope_units_kernel(const RopeRowsArgs a) {
     const long long tok = blockIdx.x / a.parts;
     const int part = blockIdx.x % a.parts;
     const int pos = a.pos ? a.pos[tok] : a.pos0 + static_cast<int>(tok);
-    for (int i = threadIdx.x; i < a.pairs; i += blockDim.x) cs[rope_slot<kLayout>(i)] = rope_turn(a.turns[i], pos, a.magnitude);
+    for (int i = threadIdx.x; i < a.pairs; i += blockDim.x) cs[rope_slot(i)] = rope_turn(a.turns[i], pos, a.magnitude);
     __syncthreads();
     const int q_units = a.q ? a.q_heads * L : 0, k_units = a.kv_heads * L;
     const int u1 = min(q_units + k_units + (a.v ? k_units : 0), (part + 1) * a.units_per_block);
