@@ -224,6 +224,11 @@ def run_reference_arm(args):
     rank = int(os.environ.get("RANK", "0"))
     if rank != 0:
         return 0
+    from oracle import oracle as orc
+    if orc.ref_lib() is None:  # this arm's number is the reference's own code or none
+        print(json.dumps({"impl": "reference", "unavailable": "the reference's sources were not there to be built "
+                                                              "(oracle/_ref/libligguf_ref.so is missing)"}), flush=True)
+        return 0
     w = DECODE_WORKLOADS[WORKLOAD]
     r = cpu_timed_steps(w, args.steps, args.warmup)
     world = int(os.environ.get("WORLD_SIZE", str(args.gpus)))
