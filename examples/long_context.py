@@ -43,7 +43,8 @@ def run(prompt=3000, chunk=700, tokens=8, draft=4, layers=2, heads=32, kv_heads=
     g = torch.Generator(device="cuda").manual_seed(seed)
     total = prompt + max(tokens, draft)
     nq, nk, row = heads * dim, kv_heads * dim, (heads + 2 * kv_heads) * dim
-    # A context four times the trained one: frequencies blended by wavelength, logits a little larger for it.
+    # A context four times the trained one: frequencies blended by wavelength, logits a little larger for it.  (A model
+    # whose ramp runs over the pairs' indices passes its own table: freq=.)
     rope = RopeConfig(dim, dim, "halves", base=1e6, scaling="blend", factor=4.0, orig_context=8192, low=1.0, high=32.0,
                       magnitude=1.1386)
     layout = dict(n_heads=heads, n_kv_heads=kv_heads)

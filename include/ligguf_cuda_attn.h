@@ -312,7 +312,9 @@ int ligguf_cuda_reduce_status(ligguf_reduce* r, void* stream);
 #define LIGGUF_ROPE_SCALE_LINEAR 1 /* f_i / factor */
 #define LIGGUF_ROPE_SCALE_BLEND 2  /* r = orig_context * f_i / (2 pi) turns within the trained context,
                                       g = clamp((r - low) / (high - low), 0, 1):
-                                      f_i * (g + (1 - g) / factor) */
+                                      f_i * (g + (1 - g) / factor).  Linear in the turns.  A model whose
+                                      ramp runs over the pair's index instead (YaRN as most GGUF models
+                                      have it) passes its own frequencies in `freq` */
 typedef struct ligguf_rope_cfg {
     int head_dim;      /* 64 or 128 */
     int rope_dim;      /* leading elements of a head that are rotated: even, 0 (none) to head_dim */
@@ -322,7 +324,8 @@ typedef struct ligguf_rope_cfg {
     float factor;      /* scaled: >= 1 */
     int orig_context;  /* BLEND: positions of the trained context */
     float low, high;   /* BLEND: low < high */
-    float magnitude;   /* multiplies the rotated elements; 0 = 1 (0.1 ln(factor) + 1 for YaRN) */
+    float magnitude;   /* multiplies the rotated elements; 0 = 1 (0.1 ln(factor) + 1 for YaRN,
+                          with whichever frequencies) */
     const float* freq; /* optional host table of rope_dim/2 inverse frequencies, used as they are in
                           place of base and scaling; NULL = computed */
 } ligguf_rope_cfg;
@@ -357,7 +360,8 @@ int ligguf_cuda_qk_rope_async(ligguf_qk_rope* h, int n, int pos0, const int* d_p
 /* A handle holds, for n_layers layers and n_seqs sequences, n_context positions of keys (normed and
  * rotated) and values in 4.5 bits: each 32 elements of a head are one block of GGUF's Q4_0 type:
  * d = fp16(m / -8) with m the element of largest magnitude (the positive one of two), codes
- * clamp(round(x / d) + 8, 0, 15), value (code - 8) * d.  |d| saturates at 65504; a block with an
+ * clamp(round(x * (1 / d)) + 8, 0, 15) with the stored d and its fp32 reciprocal (0 for d = 0), value
+ * (code - 8) * d.  |d| saturates at 65504; a block with an
  * infinity or a NaN in it becomes NaN.  In HBM the codes lie in the order in which the attention
  * kernel's matrix instructions take them; load / store convert from and to blocks.
  * One call at a time: the calls of one handle must not overlap on the GPU. */

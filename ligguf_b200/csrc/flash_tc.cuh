@@ -68,7 +68,7 @@ struct TcArgs {
 // rounding the result (bf16 1.62e-3, fp16 2.0e-4; with weights rounded once 2.13e-3 and 2.7e-4), and every
 // exponential is ex2.approx, whose error is below lo's last bit, not the cubic's.  It costs half as many products
 // again and the softmax warps' second packing: 2048 queries, window 512: 40 us against 36; 8192 queries, window 4096:
-// 540 to 620 us against 430 to 490.  The caller may choose the rounding (round_weights).
+// 540 to 630 us against 430 to 515.  The caller may choose the rounding (round_weights).
 struct TcFull {
     static constexpr bool kWindow = false, kTwoWeights = false;
     using Operand = __nv_bfloat16;

@@ -66,8 +66,10 @@ struct Kv4DecodeArgs {
 // or the later of the two would hide that a block gave up and left tickets behind.
 enum : int { kKv4ErrWait = 0, kKv4ErrPosition = 1, kKv4ErrWords = 2 };
 
-// Eight warps a block; two blocks an SM, or one of twice the registers for eight heads a KV head.  (One block of
-// sixteen warps is slower: nothing covers its starts and joins. 24 sequences: 58.8 us against 47.)
+// Eight warps a block; two blocks an SM, or one of twice the registers for eight heads a KV head (232 of them; 64 and 8
+// heads of 128: one token over 32768 positions 22.8 us, 16 sequences of 8192 64.8 us, where 32 and 8 heads take 22.8
+// and 51.4).  At 128 registers, head_dim 128 spills 112 to 124 bytes.  (One block of sixteen
+// warps is slower: nothing covers its starts and joins. 24 sequences: 58.8 us against 47.)
 __host__ __device__ constexpr int kv4_warps(int) { return 8; }
 __host__ __device__ constexpr int kv4_blocks_per_sm(int nrep) { return nrep > 4 ? 1 : 2; }
 // Units that an item counts beside its tiles and its token: what a block spends on entering and joining an

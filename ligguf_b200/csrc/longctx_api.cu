@@ -429,11 +429,18 @@ int launch_window_d(const ligguf_window* h, const lg::WindowArgs& a, cudaStream_
     // Few rows a KV head: all of them against each key tile once, the keys split over the SMs.  Up to 64 rows this
     // is bound by K and V; the tensor-core form reads them once a head and gives a head's keys to one SM.  More rows
     // go in chunks of 64 where the tensor-core form would leave most SMs without work: one of its SMs takes about
-    // 9 us for 1024 keys of a head, a chunk 20 us of one SM's time, and there is a join.  Hence the bounds of a
-    // quarter as many chunks as SMs and of 1024 keys.  Measured, 32 heads and 8 KV heads of 128, one sequence, us in
-    // chunks / on the tensor cores: 17 tokens, 512 keys 10.4 / 10.6, 1024 11.4 / 14.9, 4096 22.4 / 41.2, 32768
-    // 76.6 / 297; 64 tokens, 512 keys 12.7 / 10.7, 1024 15.2 / 15.2, 32768 135 / 297; 100 tokens (56 chunks), 2048
-    // keys 27.9 / 24.2, 32768 231 / 297.
+    // 10 us for 1024 keys of a head, a chunk 24 us of one SM's time, and there is a join.  Hence the bounds of a
+    // quarter as many chunks as SMs and of 1024 keys.  Measured, one sequence, head_dim 128, us in chunks / on the
+    // tensor cores with 1024, 4096 and 32768 keys:
+    //   32 and 8 heads   17 tokens  12.0 / 17.3   24.4 / 49.3   91.5 / 344     (rounded 11.5 / 15.2, 22.5 / 42.1, 76.9 / 297)
+    //                    64 tokens  16.2 / 17.4   34.9 / 49.5   165 / 344
+    //   16 and 16       100 tokens  15.7 / 17.4   34.1 / 50.1   164 / 346
+    //    8 and 2        288 tokens  16.6 / 18.0   33.6 / 49.4   182 / 342
+    //   16 and 2        288 tokens  18.3 / 18.3   49.6 / 49.9   345 / 344     (rounded 16.1 / 16.1, 42.0 / 42.0, 290 / 289)
+    //    4 and 1        288 tokens  14.8 / 17.9   23.5 / 49.2   98 / 342
+    // Never more than 2 % slower at 9 to 288 tokens of seven such layouts.  With 512 keys it would be (64 tokens of 32
+    // and 8 heads, rounded: 12.7 / 10.7), and so it can be where entries are that short under a large m: their lengths
+    // lie in device memory.
     const int nrep = a.q_heads / a.kv_heads;
     const long long rows = static_cast<long long>(a.n) * nrep;
     const long long keys = a.window ? std::min<long long>(a.m, static_cast<long long>(a.window) + a.n + a.sinks) : a.m;

@@ -188,9 +188,9 @@ __device__ __forceinline__ int2 rope_two_units(int dl, int pairs) {
 
 // Heads that are normed and rotated: block (token, part), a pair of units of kTake heads a thread.  Bound by the bytes
 // of the rows, each read and written once, if only enough of them are on their way.  What a thread does hangs on its
-// loads, the token's rotations (fp64, then sine and cosine: hidden by the loads) and a barrier, so it takes as many
-// heads as 64 registers hold: two of 16 bits, one of 32.  7777 tokens of 40 heads in fp16: 32.7 us (4.9 TB/s; 28 without
-// the norm); one head a thread 43, four heads, whose registers halve the threads, 36; blocks that stay and are fed by
+// loads, the token's rotations (fp64, then sine and cosine: hidden by the loads) and a barrier, so it takes about as many
+// heads as 64 registers hold: one of 32 bits, two of 16, with 24 to 72 bytes of spills.  7777 tokens of 40 heads in fp16:
+// 33 us (4.9 TB/s; 28 without the norm); one head a thread 43, four heads, whose registers halve the threads, 36; blocks that stay and are fed by
 // bulk copies into shared memory 35 to 37: shared memory's rate bounds them.
 template <typename In, typename Out, int D, int kLayout, int kTake>
 __global__ void __launch_bounds__(256, 4) rope_pairs_kernel(const RopeRowsArgs a) {

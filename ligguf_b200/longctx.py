@@ -52,13 +52,13 @@ class RopeConfig:
     rope_dim: int
     layout: str = "adjacent"  # pairs (2i, 2i+1), or "halves": (i, i + rope_dim/2)
     base: float = 10000.0
-    scaling: str = "none"     # "linear", or "blend" by the turns within orig_context
+    scaling: str = "none"     # "linear", or "blend": a ramp linear in the turns within orig_context
     factor: float = 1.0
     orig_context: int = 0
     low: float = 1.0
     high: float = 4.0
     magnitude: float = 0.0    # of the rotated elements; 0 = 1
-    freq: np.ndarray | None = None  # rope_dim/2 inverse frequencies in place of base and scaling
+    freq: np.ndarray | None = None  # rope_dim/2 inverse frequencies in place of base and scaling (other ramps: YaRN by pairs)
 
     def to_c(self):
         if self.layout not in LAYOUTS or self.scaling not in SCALINGS:
